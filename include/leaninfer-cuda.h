@@ -166,6 +166,65 @@ typedef struct li_stack_layer {
     li_ffn_weights ffn;
 } li_stack_layer;
 
+/* Element types of the activations that the rotary and append entries take
+ * (ggml's type ids). */
+#define LI_DTYPE_F32   0
+#define LI_DTYPE_F16   1
+#define LI_DTYPE_BF16  30
+
+/*
+ * Rotary position embedding. Of every head's head_dim values the first
+ * rope_dim are rotated in rope_dim/2 pairs, the rest pass through. Pair i is
+ *   LI_ROPE_INTERLEAVED  (x[2i], x[2i+1])
+ *   LI_ROPE_HALF         (x[i],  x[i + rope_dim/2])
+ * and the token at position p turns it by the angle
+ *   a   = p * theta^(-2i/rope_dim) / freq_factors[i] * (freq_scale (1-r) + r)
+ *   (y1, y2) = m (x1 cos a - x2 sin a,  x2 cos a + x1 sin a)
+ * with r = 0 and m = attn_factor, or, where ext_factor != 0 (YaRN, the
+ * published method: high frequencies keep their angle, low ones are
+ * interpolated),
+ *   r   = ext_factor * (1 - clamp((i - lo) / max(0.001, hi - lo), 0, 1))
+ *   lo  = max(0, floor(c(beta_fast))),  hi = min(rope_dim - 1, ceil(c(beta_slow)))
+ *   c(b) = rope_dim * ln(n_ctx_orig / (2 pi b)) / (2 ln theta)
+ *   m   = attn_factor * (1 + 0.1 ln(1 / freq_scale))
+ * Angles are computed in double, products and sums in fp32, one rounding to
+ * the output type.
+ */
+#define LI_ROPE_INTERLEAVED 0
+#define LI_ROPE_HALF        1
+typedef struct li_rope {
+    int   layout;        /* LI_ROPE_INTERLEAVED or LI_ROPE_HALF                */
+    int   head_dim;      /* even, 2 .. 512                                     */
+    int   rope_dim;      /* even, 0 .. head_dim                                */
+    int   n_ctx_orig;    /* YaRN: trained context length (> 0)                 */
+    float theta;         /* base of the frequencies (> 1)                      */
+    float freq_scale;    /* > 0; 1: unscaled, 1/s: interpolated for s x length */
+    float ext_factor;    /* 0: off; 1: YaRN                                    */
+    float attn_factor;   /* magnitude of the rotated values (1: none)          */
+    float beta_fast, beta_slow;   /* YaRN: turns over n_ctx_orig (> 0)         */
+    const float *freq_factors;    /* [rope_dim/2] device memory, or NULL (1)   */
+} li_rope;
+
+/*
+ * One attention layer's KV cache for a batch: every sequence's own slots,
+ * optionally a prefix that all sequences share (a common prompt, held once),
+ * and optionally what the eviction needs: the attention weight that each
+ * cached token has received and the position of the token in each slot.
+ * A token's slot and its position are separate: keys are cached rotated by
+ * their position, and the order of the slots means nothing to the attention.
+ * All pointers are device memory, k, v and the prefix 16-byte aligned.
+ */
+typedef struct li_kv_cache {
+    int n_seqs, max_ctx;           /* sequences, slots per sequence              */
+    int n_kv_heads, head_dim;      /* head_dim 128 is the only built size        */
+    void *k, *v;                   /* __half [n_seqs][max_ctx][n_kv_heads][D]    */
+    int32_t *len;                  /* [n_seqs] slots in use, 0 .. max_ctx        */
+    int n_prefix;                  /* shared tokens (0: none)                    */
+    const void *k_prefix, *v_prefix;   /* __half [n_prefix][n_kv_heads][D]       */
+    float *weight;                 /* [n_seqs][n_kv_heads][max_ctx] or NULL      */
+    int32_t *slot_pos;             /* [n_seqs][n_kv_heads][max_ctx] or NULL      */
+} li_kv_cache;
+
 #if defined(GGML_USE_CUDA) || defined(GGML_USE_CUBLAS)
 
 /* ======================================================================
@@ -381,6 +440,69 @@ int li_launch_attn_layer_decode(const li_attn_layer * L,
         const int32_t * pos, int n_seqs, int max_ctx,
         void * workspace, size_t workspace_bytes, void * stream);
 
+/* Rotary positions (see li_rope) of x [n_tokens][n_heads][head_dim]: strides
+ * in elements between tokens and between heads, the head's values contiguous.
+ * dst has its own strides and the element type of x; dst may be x itself with
+ * the same strides, and must not overlap it in any other way. pos [n_tokens]
+ * int32 in device memory, any value (a negative one turns backwards).
+ * transpose != 0 applies the transposed matrix: the gradient of the rotation,
+ * and its inverse where the magnitude m is 1. Turning cached keys by a
+ * difference of positions is the same call on the cache rows (LI_DTYPE_F16,
+ * pos = the difference). dtype LI_DTYPE_F32, _F16 or _BF16. No counterpart
+ * among the reference's kernels. */
+int li_launch_rope(const li_rope * R, int dtype, const void * x, void * dst, const int32_t * pos,
+        int n_tokens, int n_heads, int64_t x_token_stride, int64_t x_head_stride,
+        int64_t dst_token_stride, int64_t dst_head_stride, int transpose, void * stream);
+
+/* Rotates the new tokens' q and k and appends k and v to the cache. Token t
+ * belongs to sequence seq[t] (NULL: t) and goes to slot slot[t] (NULL: the
+ * last one in use, len[seq] - 1): one token per sequence at decode after the
+ * caller advanced len, or whole prompts with seq and slot given. q
+ * [n_tokens][n_q_heads][D] is written rotated to q_out (which may be q with
+ * the same stride; q NULL: no queries), k and v [n_tokens][n_kv_heads][D] are
+ * rounded to f16 into their cache rows (k rotated; R NULL: nothing rotates);
+ * strides in elements between tokens, heads contiguous. Where the cache holds
+ * them, weight is set to 0 and slot_pos to pos[t] in the new slots. len is
+ * not changed. A sequence or slot outside the cache writes nothing there and
+ * li_device_status() reports LI_ERR_BAD_ARG (its q is still rotated). Two
+ * tokens of a call must not name the same slot. R's head_dim is the cache's.
+ * No counterpart among the reference's kernels. */
+int li_launch_kv_append(const li_kv_cache * C, const li_rope * R, int dtype,
+        const void * q, int64_t q_stride, void * q_out, int64_t q_out_stride, int n_q_heads,
+        const void * k, int64_t k_stride, const void * v, int64_t v_stride,
+        const int32_t * pos, const int32_t * seq, const int32_t * slot, int n_tokens, void * stream);
+
+/* Attention of one token per sequence over the shared prefix and the
+ * sequence's own slots 0 .. len[s]-1, q head h on kv head h / (Hq / Hkv):
+ *   o[s][h] = softmax_t(scale q[s][h] . K_t) V_t  over all those tokens,
+ * out [n_seqs][n_q_heads][D] fp32; q fp32, q_stride elements between
+ * sequences, heads contiguous. The prefix is read once for the whole batch. A
+ * sequence without any token gets zeros. If the cache holds weight, every own
+ * slot's weight becomes decay * weight + the sum over the kv head's q heads of
+ * its softmax probability (decay 1: accumulated, 0: replaced); slots past
+ * len[s] are left alone. A length outside 0 .. max_ctx is taken as 0 own
+ * slots and li_device_status() reports LI_ERR_BAD_ARG. Hq / Hkv in 1 .. 16;
+ * q, out 16-byte aligned, q_stride a multiple of 4. No counterpart among the
+ * reference's kernels. */
+size_t li_attn_kv_workspace_size(const li_kv_cache * C, int n_q_heads);
+int li_launch_attn_kv_decode(const li_kv_cache * C, const float * q, int64_t q_stride, int n_q_heads,
+        float scale, float * out, float decay, void * workspace, size_t workspace_bytes, void * stream);
+
+/* Shrinks every sequence of more than `budget` own slots to `budget`, for each
+ * kv head by itself. Kept are the slots whose token position (slot_pos) is
+ * below n_prefix + n_sink (the first own tokens follow the prefix) or above
+ * pos[s] - n_recent (pos[s]: the newest token's position), then those of the largest weight (a negative one or NaN counts as
+ * 0), ties going to the lowest slot; exactly `budget` in all. Slots below
+ * `budget` that are not kept are refilled in ascending order with the kept
+ * slots from `budget` on, in ascending order (K and V row, weight, slot_pos);
+ * every other row stays where it is, slots from `budget` on keep what they
+ * held, and len[s] becomes budget. Needs weight and slot_pos; n_sink +
+ * n_recent <= budget <= max_ctx. Lengths outside 0 .. max_ctx are left alone
+ * and reported as above. No counterpart among the reference's kernels. */
+size_t li_kv_evict_workspace_size(const li_kv_cache * C, int budget);
+int li_launch_kv_evict(const li_kv_cache * C, const int32_t * pos, int budget, int n_sink, int n_recent,
+        void * workspace, size_t workspace_bytes, void * stream);
+
 /* ----------------------------------------------------------------------
  * Multi-GPU: the SwiGLU FFN sharded two ways over NCCL (no counterpart in
  * the reference, which has no multi-GPU code). Sequences stay sharded by rank
@@ -539,6 +661,23 @@ static inline int li_launch_attn_layer_decode(const li_attn_layer*L, const float
         const int32_t*p, int n, int c, void*ws, size_t wb, void*s)
         {(void)L;(void)x;(void)y;(void)kc;(void)vc;(void)p;(void)n;(void)c;(void)ws;(void)wb;(void)s;
          return LI_ERR_NO_CUDA;}
+static inline int li_launch_rope(const li_rope*R, int t, const void*x, void*d, const int32_t*p, int n, int h,
+        int64_t xt, int64_t xh, int64_t dt, int64_t dh, int tr, void*s)
+        {(void)R;(void)t;(void)x;(void)d;(void)p;(void)n;(void)h;(void)xt;(void)xh;(void)dt;(void)dh;(void)tr;(void)s;
+         return LI_ERR_NO_CUDA;}
+static inline int li_launch_kv_append(const li_kv_cache*C, const li_rope*R, int t, const void*q, int64_t qs, void*qo,
+        int64_t qos, int hq, const void*k, int64_t ks, const void*v, int64_t vs, const int32_t*p, const int32_t*sq,
+        const int32_t*sl, int n, void*s)
+        {(void)C;(void)R;(void)t;(void)q;(void)qs;(void)qo;(void)qos;(void)hq;(void)k;(void)ks;(void)v;(void)vs;
+         (void)p;(void)sq;(void)sl;(void)n;(void)s; return LI_ERR_NO_CUDA;}
+static inline size_t li_attn_kv_workspace_size(const li_kv_cache*C, int h) {(void)C;(void)h; return 0;}
+static inline int li_launch_attn_kv_decode(const li_kv_cache*C, const float*q, int64_t qs, int h, float sc, float*o,
+        float d, void*ws, size_t wb, void*s)
+        {(void)C;(void)q;(void)qs;(void)h;(void)sc;(void)o;(void)d;(void)ws;(void)wb;(void)s; return LI_ERR_NO_CUDA;}
+static inline size_t li_kv_evict_workspace_size(const li_kv_cache*C, int b) {(void)C;(void)b; return 0;}
+static inline int li_launch_kv_evict(const li_kv_cache*C, const int32_t*p, int b, int ns, int nr, void*ws, size_t wb,
+        void*s)
+        {(void)C;(void)p;(void)b;(void)ns;(void)nr;(void)ws;(void)wb;(void)s; return LI_ERR_NO_CUDA;}
 static inline int li_nccl_available(void) { return 0; }
 static inline int li_nccl_get_unique_id(void*id) {(void)id; return LI_ERR_NO_CUDA;}
 static inline int li_nccl_comm_init_rank(void**c, int n, const void*id, int r)

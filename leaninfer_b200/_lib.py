@@ -78,7 +78,29 @@ class StackLayer(ctypes.Structure):
     ]
 
 
+class RopeParams(ctypes.Structure):
+    """Mirror of ``li_rope``."""
+
+    _fields_ = [
+        ("layout", c_int), ("head_dim", c_int), ("rope_dim", c_int), ("n_ctx_orig", c_int),
+        ("theta", c_float), ("freq_scale", c_float), ("ext_factor", c_float), ("attn_factor", c_float),
+        ("beta_fast", c_float), ("beta_slow", c_float), ("freq_factors", c_void_p),
+    ]
+
+
+class KvCache(ctypes.Structure):
+    """Mirror of ``li_kv_cache``."""
+
+    _fields_ = [
+        ("n_seqs", c_int), ("max_ctx", c_int), ("n_kv_heads", c_int), ("head_dim", c_int), ("k", c_void_p),
+        ("v", c_void_p), ("len", c_void_p), ("n_prefix", c_int), ("k_prefix", c_void_p), ("v_prefix", c_void_p),
+        ("weight", c_void_p), ("slot_pos", c_void_p),
+    ]
+
+
 LI_LAYER_DELTANET, LI_LAYER_ATTN = 1, 2
+LI_ROPE_INTERLEAVED, LI_ROPE_HALF = 0, 1
+LI_DTYPE_F32, LI_DTYPE_F16, LI_DTYPE_BF16 = 0, 1, 30
 
 
 class GgmlTensor(ctypes.Structure):
@@ -139,6 +161,18 @@ _SIGS = {
     "li_attn_layer_workspace_size": (c_size_t, [POINTER(AttnLayer), c_int, c_int]),
     "li_launch_attn_layer_decode": (
         c_int, [POINTER(AttnLayer)] + [c_void_p] * 5 + [c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "li_launch_rope": (
+        c_int, [POINTER(RopeParams), c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_int64,
+                c_int64, c_int, c_void_p]),
+    "li_launch_kv_append": (
+        c_int, [POINTER(KvCache), POINTER(RopeParams), c_int, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p,
+                c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "li_attn_kv_workspace_size": (c_size_t, [POINTER(KvCache), c_int]),
+    "li_launch_attn_kv_decode": (
+        c_int, [POINTER(KvCache), c_void_p, c_int64, c_int, c_float, c_void_p, c_float, c_void_p, c_size_t, c_void_p]),
+    "li_kv_evict_workspace_size": (c_size_t, [POINTER(KvCache), c_int]),
+    "li_launch_kv_evict": (
+        c_int, [POINTER(KvCache), c_void_p, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "li_nccl_available": (c_int, []),
     "li_nccl_get_unique_id": (c_int, [c_void_p]),
     "li_nccl_comm_init_rank": (c_int, [POINTER(c_void_p), c_int, c_void_p, c_int]),

@@ -11,6 +11,9 @@ int li_tu_status_prefill(int clear);
 int li_tu_status_gemm_bf16(int clear);
 int li_tu_status_selftest(int clear);
 int li_tu_status_attn(int clear);
+int li_tu_status_rope(int clear);
+int li_tu_status_kvattn(int clear);
+int li_tu_status_kvevict(int clear);
 
 namespace li {
 
@@ -112,6 +115,9 @@ int li_device_status(void) {
     if ((v = li_tu_status_gemm_bf16(1)) && !s) s = v;
     if ((v = li_tu_status_selftest(1)) && !s) s = v;
     if ((v = li_tu_status_attn(1)) && !s) s = v;
+    if ((v = li_tu_status_rope(1)) && !s) s = v;
+    if ((v = li_tu_status_kvattn(1)) && !s) s = v;
+    if ((v = li_tu_status_kvevict(1)) && !s) s = v;
     return s;
 }
 

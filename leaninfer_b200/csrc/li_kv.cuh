@@ -1,0 +1,54 @@
+// Shared pieces of the KV-cache operators (li_rope.cu, li_kvattn.cu,
+// li_kvevict.cu): the host check of a cache descriptor and the rotary
+// parameters in the form the kernels read.
+#pragma once
+#include "li_common.cuh"
+
+namespace li {
+
+constexpr int kKvD = 128;              // head_dim of the cache (the only built size)
+constexpr int kRopeMaxDim = 512;
+
+// 0, or the status a bad descriptor is refused with. Lengths live on the
+// device and are checked by the kernels.
+inline int check_kv_cache(const li_kv_cache *C) {
+    if (!C || C->n_seqs < 0 || C->max_ctx <= 0 || C->n_kv_heads <= 0 || C->n_prefix < 0) return LI_ERR_BAD_ARG;
+    if (!C->k || !C->v || !C->len) return LI_ERR_BAD_ARG;
+    if (C->n_prefix > 0 && (!C->k_prefix || !C->v_prefix)) return LI_ERR_BAD_ARG;
+    if (C->head_dim != kKvD) return LI_ERR_UNSUPPORTED;
+    if (!aligned16(C->k) || !aligned16(C->v)) return LI_ERR_MISALIGNED;
+    if (C->n_prefix > 0 && (!aligned16(C->k_prefix) || !aligned16(C->v_prefix))) return LI_ERR_MISALIGNED;
+    if (((uintptr_t)C->len & 3u) || ((uintptr_t)C->weight & 3u) || ((uintptr_t)C->slot_pos & 3u))
+        return LI_ERR_MISALIGNED;
+    // (sequence, kv head, slot) counts stay below 2^40, (sequence, kv head) pairs below 2^31
+    if ((int64_t)C->n_seqs * C->n_kv_heads >= (1ll << 31)) return LI_ERR_BAD_SHAPE;
+    return 0;
+}
+
+// li_rope as the kernels read it: the frequency of pair i in turns per
+// position (angle / 2 pi), scaling included, divided by freq_factors[i] on
+// the device.
+struct RopeArgs {
+    int layout, rope_dim;
+    float mag;                         // magnitude m of the rotated values
+    const float *factors;              // [rope_dim / 2] or nullptr
+    double turns[kRopeMaxDim / 2];
+};
+
+// Fills *a from R; 0 or a status.
+int rope_args(const li_rope *R, RopeArgs *a);
+
+// cos and sin of pair i of the token at position pos, times the magnitude.
+// The turn count is reduced to (-1/2, 1/2] in double, so the float argument
+// of sincospif carries 24 bits of the angle at any position: the error is
+// that of an angle known to 2^-25 of a half turn, whatever the position.
+__device__ __forceinline__ float2 rope_cos_sin(const RopeArgs &a, int pos, int i) {
+    double t = (double)pos * a.turns[i];
+    if (a.factors) t /= (double)a.factors[i];
+    t -= rint(t);
+    float sn, cs;
+    sincospif((float)(2.0 * t), &sn, &cs);
+    return make_float2(cs * a.mag, sn * a.mag);
+}
+
+}  // namespace li

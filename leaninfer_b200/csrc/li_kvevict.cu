@@ -1,0 +1,254 @@
+// Eviction from a KV cache by accumulated attention weight.
+//
+// For each (sequence, kv head) with more than `budget` slots in use: keep the
+// `budget` slots with the largest key, where the key is the weight's bit
+// pattern (non-negative floats order as unsigned integers; negative and NaN
+// count as 0) and 0xFFFFFFFF for the protected ones (n_sink first and n_recent
+// newest positions), ties going to the lowest slot; then fill the freed slots
+// below `budget`, ascending, with the kept ones behind it, ascending. Only
+// those rows move: sources lie at or past `budget`, destinations below it, so
+// all moves are independent and need no order.
+//
+//   kv_select   block per (sequence, kv head): the budget-th largest key by a
+//               radix search over four 8-bit digits, then the two ascending
+//               lists by warp ballots and a block scan;
+//   kv_move     warps over all lists: 512 bytes (K and V row) per move, plus
+//               weight and position.
+#include "li_kv.cuh"
+
+LI_DEFINE_TU_STATUS(kvevict)
+
+namespace li {
+namespace {
+
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / kWarp;
+constexpr int kSelCacheMax = 48 * 1024;     // keys held in shared memory up to this many slots
+
+struct EvictArgs {
+    const float *weight;
+    const int32_t *slot_pos, *pos;
+    int32_t *len;
+    int Hkv, max_ctx, budget, n_recent, max_moves;
+    int64_t first_free;                // positions below are protected: the prefix's and the sinks'
+    int32_t *count;                    // [n_seqs * Hkv] moves
+    int2 *list;                        // [n_seqs * Hkv][max_moves] (from, to)
+    __half *k, *v;
+    float *weight_rw;
+    int32_t *slot_pos_rw;
+    int n_pairs;
+};
+
+__device__ __forceinline__ uint32_t evict_key(float w, int p, int64_t first_free, int64_t newest_free) {
+    if (p < first_free || (int64_t)p > newest_free) return 0xffffffffu;
+    return w > 0.f ? __float_as_uint(w) : 0u;
+}
+
+// Exclusive scan of v over the block's warps (one value per warp, given by
+// every lane); returns this warp's offset and the total.
+__device__ __forceinline__ int warp_offsets(int v, int *buf, int &total) {
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    __syncthreads();
+    if (lane == 0) buf[warp] = v;
+    __syncthreads();
+    int off = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < kSelWarps; ++w) {
+        const int x = buf[w];
+        if (w < warp) off += x;
+        sum += x;
+    }
+    total = sum;
+    return off;
+}
+
+__global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictArgs a, bool cached) {
+    extern __shared__ uint32_t keys[];             // [max_ctx] when cached
+    __shared__ int hist[256];
+    __shared__ int buf[kSelWarps];
+    __shared__ uint32_t s_digit;
+    __shared__ int s_want;
+    grid_dep_wait();
+    grid_dep_launch_dependents();
+    const int pair = blockIdx.x, s = pair / a.Hkv;
+    const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
+    const int n = a.len[s];
+    if (n < 0 || n > a.max_ctx) {
+        if (tid == 0) {
+            atomicExch(&g_device_error, LI_ERR_BAD_ARG);
+            a.count[pair] = 0;
+        }
+        return;
+    }
+    if (n <= a.budget) {
+        if (tid == 0) a.count[pair] = 0;
+        return;
+    }
+    const float *w = a.weight + (size_t)pair * a.max_ctx;
+    const int32_t *sp = a.slot_pos + (size_t)pair * a.max_ctx;
+    const int64_t newest_free = (int64_t)a.pos[s] - a.n_recent;
+    auto key_of = [&](int i) -> uint32_t {
+        return cached ? keys[i] : evict_key(w[i], sp[i], a.first_free, newest_free);
+    };
+    if (cached)
+        for (int i = tid; i < n; i += kSelThreads) keys[i] = evict_key(w[i], sp[i], a.first_free, newest_free);
+
+    // the budget-th largest key, digit by digit from the top: `prefix` holds
+    // the digits found, `want` the rank left among the keys that share them
+    uint32_t prefix = 0, mask = 0;
+    int want = a.budget;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kSelThreads) {
+            const uint32_t k = key_of(i);
+            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            int left = want, d = 255;
+            while (d > 0 && hist[d] < left) left -= hist[d--];
+            s_digit = (uint32_t)d;
+            s_want = left;
+        }
+        __syncthreads();
+        prefix |= s_digit << shift;
+        mask |= 255u << shift;
+        want = s_want;
+        __syncthreads();
+    }
+    // keys above `prefix` are kept, of those equal to it the first `want`. A
+    // warp owns whole groups of 32 slots, in order.
+    const int groups = (n + 31) / 32, per = (groups + kSelWarps - 1) / kSelWarps;
+    const int g0 = min(warp * per, groups), g1 = min(g0 + per, groups);
+    int ties = 0;
+    for (int g = g0; g < g1; ++g) {
+        const int i = g * 32 + lane;
+        ties += __popc(__ballot_sync(0xffffffffu, i < n && key_of(i) == prefix));
+    }
+    int total;
+    const int tie0 = warp_offsets(ties, buf, total);
+    // pass 0 counts this warp's freed and moving slots, pass 1 writes them
+    int hole_at = 0, from_at = 0, moves = 0;
+    int2 *list = a.list + (size_t)pair * a.max_moves;
+    for (int pass = 0; pass < 2; ++pass) {
+        int tie = tie0, holes = hole_at, froms = from_at;
+        for (int g = g0; g < g1; ++g) {
+            const int i = g * 32 + lane;
+            const uint32_t k = i < n ? key_of(i) : 0u;
+            const bool eq = i < n && k == prefix;
+            const uint32_t eqs = __ballot_sync(0xffffffffu, eq), below = (1u << lane) - 1u;
+            const bool keep = i < n && (k > prefix || (eq && tie + __popc(eqs & below) < want));
+            tie += __popc(eqs);
+            const bool hole = i < a.budget && !keep, from = i >= a.budget && keep;   // budget < n
+            const uint32_t hb = __ballot_sync(0xffffffffu, hole), fb = __ballot_sync(0xffffffffu, from);
+            if (pass == 1) {
+                if (hole) list[holes + __popc(hb & below)].y = i;
+                if (from) list[froms + __popc(fb & below)].x = i;
+            }
+            holes += __popc(hb);
+            froms += __popc(fb);
+        }
+        if (pass == 0) {
+            hole_at = warp_offsets(holes, buf, moves);
+            from_at = warp_offsets(froms, buf, moves);     // as many kept behind the budget as freed below it
+        }
+    }
+    if (tid == 0) a.count[pair] = moves;
+}
+
+constexpr int kMoveWarps = 8, kMovePer = 4;        // moves of a warp in flight
+constexpr int kMoveChunk = kMoveWarps * kMovePer;  // moves per block and step
+
+__global__ void __launch_bounds__(kMoveWarps * kWarp) kv_move_kernel(EvictArgs a, int chunks) {
+    grid_dep_wait();
+    grid_dep_launch_dependents();
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    const int64_t items = (int64_t)a.n_pairs * chunks;
+    for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+        const int pair = (int)(it / chunks), chunk = (int)(it % chunks);
+        const int s = pair / a.Hkv, j = pair % a.Hkv;
+        const int n = a.count[pair];
+        if (chunk == 0 && j == 0 && threadIdx.x == 0 && a.len[s] > a.budget && a.len[s] <= a.max_ctx)
+            a.len[s] = a.budget;
+        const int m0 = chunk * kMoveChunk + warp * kMovePer;
+        if (m0 >= n) continue;
+        const int2 *list = a.list + (size_t)pair * a.max_moves;
+        // lanes 0-15 carry the K row, 16-31 the V row, 16 bytes each
+        __half *base = (lane < 16 ? a.k : a.v) + ((size_t)s * a.max_ctx * a.Hkv + j) * kKvD + (lane & 15) * 8;
+        const size_t stride = (size_t)a.Hkv * kKvD;
+        int2 mv[kMovePer];
+        uint4 d[kMovePer];
+#pragma unroll
+        for (int i = 0; i < kMovePer; ++i)
+            if (m0 + i < n) mv[i] = list[m0 + i];
+#pragma unroll
+        for (int i = 0; i < kMovePer; ++i)
+            if (m0 + i < n) d[i] = *reinterpret_cast<const uint4 *>(base + (size_t)mv[i].x * stride);
+#pragma unroll
+        for (int i = 0; i < kMovePer; ++i)
+            if (m0 + i < n) *reinterpret_cast<uint4 *>(base + (size_t)mv[i].y * stride) = d[i];
+        if (lane < kMovePer && m0 + lane < n) {
+            const int2 m = list[m0 + lane];
+            const size_t at = (size_t)pair * a.max_ctx;
+            a.weight_rw[at + m.y] = a.weight_rw[at + m.x];
+            a.slot_pos_rw[at + m.y] = a.slot_pos_rw[at + m.x];
+        }
+    }
+}
+
+size_t al256(size_t v) { return (v + 255) / 256 * 256; }
+
+int moves_max(const li_kv_cache *C, int budget) {
+    return budget < C->max_ctx - budget ? budget : C->max_ctx - budget;
+}
+
+}  // namespace
+}  // namespace li
+
+using namespace li;
+
+extern "C" {
+
+size_t li_kv_evict_workspace_size(const li_kv_cache *C, int budget) {
+    if (check_kv_cache(C) || C->n_seqs == 0 || budget < 0 || budget > C->max_ctx) return 0;
+    const size_t pairs = (size_t)C->n_seqs * C->n_kv_heads;
+    return al256(pairs * sizeof(int32_t)) + al256(pairs * (size_t)moves_max(C, budget) * sizeof(int2));
+}
+
+int li_launch_kv_evict(const li_kv_cache *C, const int32_t *pos, int budget, int n_sink, int n_recent,
+                       void *workspace, size_t workspace_bytes, void *stream) {
+    if (const int rc = check_kv_cache(C)) return rc;
+    if (!pos || !C->weight || !C->slot_pos || budget < 0 || n_sink < 0 || n_recent < 0) return LI_ERR_BAD_ARG;
+    if (budget > C->max_ctx || (int64_t)n_sink + n_recent > budget) return LI_ERR_BAD_SHAPE;
+    if ((uintptr_t)pos & 3u) return LI_ERR_MISALIGNED;
+    if (C->n_seqs == 0) return 0;
+    if (!workspace || workspace_bytes < li_kv_evict_workspace_size(C, budget)) return LI_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return LI_ERR_MISALIGNED;
+    EvictArgs a = {};
+    const int pairs = C->n_seqs * C->n_kv_heads;
+    a.weight = C->weight; a.slot_pos = C->slot_pos; a.pos = pos; a.len = C->len;
+    a.Hkv = C->n_kv_heads; a.max_ctx = C->max_ctx; a.budget = budget; a.first_free = (int64_t)C->n_prefix + n_sink; a.n_recent = n_recent;
+    a.max_moves = moves_max(C, budget);
+    a.count = static_cast<int32_t *>(workspace);
+    a.list = reinterpret_cast<int2 *>(static_cast<char *>(workspace) + al256((size_t)pairs * sizeof(int32_t)));
+    a.k = static_cast<__half *>(C->k); a.v = static_cast<__half *>(C->v);
+    a.weight_rw = C->weight; a.slot_pos_rw = C->slot_pos;
+    a.n_pairs = pairs;
+    const cudaStream_t st = (cudaStream_t)stream;
+    const bool cached = C->max_ctx <= kSelCacheMax;
+    const size_t smem = cached ? (size_t)C->max_ctx * 4 : 0;
+    if (smem > 40 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kv_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   kSelCacheMax * 4);
+        if (e != cudaSuccess) return (int)e;
+    }
+    int rc = (int)launch_pdl(kv_select_kernel, dim3((unsigned)pairs), dim3(kSelThreads), smem, st, true, a, cached);
+    if (rc) return rc;
+    const int chunks = a.max_moves > 0 ? (a.max_moves + kMoveChunk - 1) / kMoveChunk : 1;
+    const int64_t items = (int64_t)pairs * chunks, cap = (int64_t)num_sms() * 8;
+    return (int)launch_pdl(kv_move_kernel, dim3((unsigned)(items < cap ? items : cap)), dim3(kMoveWarps * kWarp), 0,
+                           st, true, a, chunks);
+}
+
+}  // extern "C"

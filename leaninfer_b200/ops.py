@@ -15,13 +15,15 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import (LI_WTYPE_Q4_K, LI_WTYPE_Q8_0, AttnLayer, DeltaNetLayer, LeanInferError, check)
+from ._lib import (LI_DTYPE_BF16, LI_DTYPE_F16, LI_DTYPE_F32, LI_ROPE_HALF, LI_ROPE_INTERLEAVED, LI_WTYPE_Q4_K,
+                   LI_WTYPE_Q8_0, AttnLayer, DeltaNetLayer, KvCache, LeanInferError, RopeParams, check)
 
 __all__ = [
     "rms_norm_matmul_f32", "rms_norm_swiglu_f32", "rms_norm_swiglu_f16", "rms_norm_qkv_f32",
     "rms_norm_silu_gate_f32", "deltanet_recurrent_out_f32", "deltanet_recurrent_f32",
     "dequantize", "rms_norm_matmul_q", "rms_norm_qkv_q", "rms_norm_swiglu_q", "ffn_q",
-    "DeltaNetLayerDecode", "AttnLayerDecode", "device_status", "row_bytes", "LI_WTYPE_Q8_0", "LI_WTYPE_Q4_K",
+    "DeltaNetLayerDecode", "AttnLayerDecode", "Rope", "rope", "KVCache", "device_status", "row_bytes",
+    "LI_WTYPE_Q8_0", "LI_WTYPE_Q4_K",
 ]
 
 
@@ -317,3 +319,184 @@ class AttnLayerDecode:
             ctypes.byref(self.L), _p(x), _p(y), _p(k_cache), _p(v_cache), _p(pos), n_seqs, max_ctx, _p(ws),
             ws.numel(), _stream()), "li_launch_attn_layer_decode")
         return y
+
+
+# --------------------------------------------------------------------------
+# Rotary positions and the managed KV cache
+# --------------------------------------------------------------------------
+_DTYPES = {torch.float32: LI_DTYPE_F32, torch.float16: LI_DTYPE_F16, torch.bfloat16: LI_DTYPE_BF16}
+_ROPE_LAYOUTS = {"interleaved": LI_ROPE_INTERLEAVED, "half": LI_ROPE_HALF}
+
+
+def _dev(device: torch.device, *tensors, dtype=None) -> None:
+    """The tensors lie on `device`, and it is the current one (the library
+    launches on the current device's stream)."""
+    if device.type != "cuda":
+        raise ValueError("LeanInfer kernels take CUDA tensors")
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {device}, but cuda:{torch.cuda.current_device()} is the current device")
+    for t in tensors:
+        if t is not None:
+            if t.device != device:
+                raise ValueError(f"tensors on {t.device} and {device}")
+            if dtype is not None and t.dtype != dtype:
+                raise ValueError(f"expected {dtype}, got {t.dtype}")
+
+
+def _heads(t: torch.Tensor, n: int, heads: int | None, dim: int, what: str) -> None:
+    """[n, heads, dim] with each token's heads contiguous; any token stride."""
+    if t.dim() != 3 or t.shape[0] != n or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{what}: expected [{n}, {heads or 'heads'}, {dim}], got {tuple(t.shape)}")
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim):
+        raise ValueError(f"{what}: the heads of a token must be contiguous")
+
+
+def _index(t: torch.Tensor | None, n: int, what: str) -> int | None:
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous int32 tensor of {n} values")
+    return t.data_ptr()
+
+
+class Rope:
+    """Rotary position parameters (li_rope): layout "half" or "interleaved",
+    the first rope_dim dims of head_dim, position interpolation (freq_scale)
+    and YaRN (ext_factor 1 with n_ctx_orig, beta_fast, beta_slow),
+    freq_factors an fp32 device tensor of rope_dim / 2 divisors or None."""
+
+    def __init__(self, *, head_dim: int, rope_dim: int | None = None, layout: str = "half", theta: float = 1e7,
+                 freq_scale: float = 1.0, ext_factor: float = 0.0, attn_factor: float = 1.0, beta_fast: float = 32.0,
+                 beta_slow: float = 1.0, n_ctx_orig: int = 0, freq_factors: torch.Tensor | None = None):
+        rope_dim = head_dim if rope_dim is None else rope_dim
+        if layout not in _ROPE_LAYOUTS:
+            raise ValueError(f"layout {layout!r}: expected one of {sorted(_ROPE_LAYOUTS)}")
+        if freq_factors is not None and (freq_factors.dtype != torch.float32 or freq_factors.numel() != rope_dim // 2):
+            raise ValueError(f"freq_factors: expected {rope_dim // 2} fp32 values")
+        self.keep = freq_factors
+        self.R = RopeParams(layout=_ROPE_LAYOUTS[layout], head_dim=head_dim, rope_dim=rope_dim, n_ctx_orig=n_ctx_orig,
+                            theta=theta, freq_scale=freq_scale, ext_factor=ext_factor, attn_factor=attn_factor,
+                            beta_fast=beta_fast, beta_slow=beta_slow, freq_factors=_p(freq_factors))
+        self.head_dim = head_dim
+        self.ref = ctypes.byref(self.R)
+
+
+def rope(rope: Rope, x: torch.Tensor, pos: torch.Tensor, out: torch.Tensor | None = None, transpose: bool = False):
+    """x [tokens, heads, head_dim] (fp32, fp16 or bf16; any token and head
+    strides) rotated to the positions pos (int32 [tokens]); transpose: the
+    transposed rotation (its gradient). out may be x."""
+    n, heads, dim = x.shape
+    if dim != rope.head_dim or x.stride(2) != 1:
+        raise ValueError(f"x: expected [tokens, heads, {rope.head_dim}] with contiguous heads")
+    if out is None:
+        out = torch.empty(n, heads, dim, device=x.device, dtype=x.dtype)
+    elif out.shape != x.shape or out.stride(2) != 1:
+        raise ValueError("out: expected the shape of x with contiguous heads")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"x: {x.dtype} is not fp32, fp16 or bf16")
+    _dev(x.device, out, dtype=x.dtype)
+    _dev(x.device, pos, rope.keep)
+    check(_lib.load().li_launch_rope(rope.ref, _DTYPES[x.dtype], x.data_ptr(), out.data_ptr(), _index(pos, n, "pos"),
+                                     n, heads, x.stride(0), x.stride(1), out.stride(0), out.stride(1), int(transpose),
+                                     _stream()), "li_launch_rope")
+    return out
+
+
+class KVCache:
+    """One attention layer's KV cache (li_kv_cache) over the caller's tensors:
+    k, v fp16 [n_seqs, max_ctx, n_kv_heads, 128]; len int32 [n_seqs], the slots
+    in use, which the caller advances before a step's append; an optional
+    shared prefix fp16 [n_prefix, n_kv_heads, 128]; weight fp32 and slot_pos
+    int32 [n_seqs, n_kv_heads, max_ctx] for the eviction. Workspaces are kept
+    by the object; calls that overlap on the GPU need an object each."""
+
+    def __init__(self, k, v, len, *, k_prefix=None, v_prefix=None, weight=None, slot_pos=None):
+        n, ctx, heads, dim = k.shape
+        self.device = k.device
+        if v.shape != k.shape:
+            raise ValueError("k and v differ in shape")
+        if (k_prefix is None) != (v_prefix is None):
+            raise ValueError("k_prefix and v_prefix go together")
+        p = 0 if k_prefix is None else k_prefix.shape[0]
+        if p and (tuple(k_prefix.shape) != (p, heads, dim) or v_prefix.shape != k_prefix.shape):
+            raise ValueError(f"prefix: expected [n_prefix, {heads}, {dim}]")
+        for t, dt in ((weight, torch.float32), (slot_pos, torch.int32)):
+            if t is not None and (tuple(t.shape) != (n, heads, ctx) or t.dtype != dt):
+                raise ValueError(f"weight and slot_pos: expected fp32 and int32 [{n}, {heads}, {ctx}]")
+        for t in (k, v, k_prefix, v_prefix):
+            if t is not None and t.dtype != torch.float16:
+                raise ValueError("the cache rows are fp16")
+        self.keep = [k, v, len, k_prefix, v_prefix, weight, slot_pos]
+        for t in self.keep:
+            if t is not None and t.device != k.device:
+                raise ValueError(f"tensors on {t.device} and {k.device}")
+        self.n_seqs, self.max_ctx, self.n_kv_heads, self.head_dim = n, ctx, heads, dim
+        self.C = KvCache(n_seqs=n, max_ctx=ctx, n_kv_heads=heads, head_dim=dim, k=_p(k), v=_p(v),
+                         len=_index(len, n, "len"), n_prefix=p, k_prefix=_p(k_prefix) if p else None,
+                         v_prefix=_p(v_prefix) if p else None, weight=_p(weight), slot_pos=_p(slot_pos))
+        self.ref = ctypes.byref(self.C)
+        self._ws = {}
+
+    def _workspace(self, key, size) -> torch.Tensor:
+        ws = self._ws.get(key)
+        if ws is None:
+            ws = self._ws[key] = torch.empty(max(size(), 16), device=self.device, dtype=torch.uint8)
+        return ws
+
+    def append(self, k, v, pos, *, q=None, rope: Rope | None = None, seq=None, slot=None, q_out=None):
+        """Appends k, v [tokens, n_kv_heads, 128] (k rotated to pos) at
+        (seq[t], slot[t]); without seq, token t is sequence t's, without slot
+        it goes to slot len - 1. Returns q rotated (q_out, which may be q), or
+        None without q."""
+        n = k.shape[0]
+        if k.dtype not in _DTYPES:
+            raise ValueError(f"k: {k.dtype} is not fp32, fp16 or bf16")
+        _heads(k, n, self.n_kv_heads, self.head_dim, "k")
+        _heads(v, n, self.n_kv_heads, self.head_dim, "v")
+        _dev(self.device, k, v, q, q_out, dtype=k.dtype)
+        _dev(self.device, pos, seq, slot, rope.keep if rope is not None else None)
+        qp = op = None
+        qs = os = hq = 0
+        if q is not None:
+            hq = q.shape[1]
+            _heads(q, n, hq, self.head_dim, "q")
+            if q_out is None:
+                q_out = torch.empty(n, hq, self.head_dim, device=self.device, dtype=q.dtype)
+            else:
+                _heads(q_out, n, hq, self.head_dim, "q_out")
+            qp, op, qs, os = q.data_ptr(), q_out.data_ptr(), q.stride(0), q_out.stride(0)
+        check(_lib.load().li_launch_kv_append(
+            self.ref, rope.ref if rope is not None else None, _DTYPES[k.dtype], qp, qs, op, os, hq, k.data_ptr(),
+            k.stride(0), v.data_ptr(), v.stride(0), _index(pos, n, "pos"), _index(seq, n, "seq"),
+            _index(slot, n, "slot"), n, _stream()), "li_launch_kv_append")
+        return q_out if q is not None else None
+
+    def decode(self, q, *, scale: float | None = None, decay: float = 1.0, out=None, workspace=None):
+        """Attention of q [n_seqs, n_q_heads, 128] (fp32) over the prefix and
+        each sequence's first len slots; returns [n_seqs, n_q_heads, 128]. With
+        weight in the cache, weight = decay * weight + this step's."""
+        _heads(q, self.n_seqs, None, self.head_dim, "q")
+        hq = q.shape[1]
+        if out is None:
+            out = torch.empty(self.n_seqs, hq, self.head_dim, device=self.device, dtype=torch.float32)
+        elif out.shape != q.shape or not out.is_contiguous():
+            raise ValueError("out: expected a contiguous tensor of q's shape")
+        _dev(self.device, q, out, dtype=torch.float32)
+        lib = _lib.load()
+        ws = workspace if workspace is not None else self._workspace(
+            hq, lambda: int(lib.li_attn_kv_workspace_size(self.ref, hq)))
+        check(lib.li_launch_attn_kv_decode(self.ref, q.data_ptr(), q.stride(0), hq,
+                                           self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), decay,
+                                           ws.data_ptr(), ws.numel(), _stream()), "li_launch_attn_kv_decode")
+        return out
+
+    def evict(self, pos, budget: int, *, n_sink: int = 0, n_recent: int = 0, workspace=None) -> None:
+        """Shrinks every longer sequence to `budget` slots by weight (see
+        li_launch_kv_evict); pos int32 [n_seqs], the newest token's position;
+        n_sink counts own tokens, after the prefix."""
+        _dev(self.device, pos)
+        lib = _lib.load()
+        ws = workspace if workspace is not None else self._workspace(
+            ("evict", budget), lambda: int(lib.li_kv_evict_workspace_size(self.ref, budget)))
+        check(lib.li_launch_kv_evict(self.ref, _index(pos, self.n_seqs, "pos"), budget, n_sink, n_recent,
+                                     ws.data_ptr(), ws.numel(), _stream()), "li_launch_kv_evict")
