@@ -1,89 +1,1143 @@
 // Attention of one token per sequence over a shared prefix and the
 // sequence's own cache slots, with the accumulation of each own slot's
 // attention weight.
+//
+//   o[s][h] = softmax_t(scale q[s][h] . K_t) V_t,  t over prefix and own slots
+//   weight[s][j][t] = decay weight + sum_g p[s][jG+g][t]      (own slots)
+//
+// Both parts are cut along the tokens into pieces that fill the SMs evenly;
+// a piece leaves (max, sum, o[128]) per q head, and the last kernel joins
+// them. Every product takes q and p as two f16 parts (hi + lo: 22 bits), since
+// K and V are f16 already: twice the tensor work of one part, for outputs that
+// are as exact as fp32 sums (one part would leave 2^-12). Probabilities carry
+// a factor 2^7, so that the lo part of a probability far below the largest is
+// still a normal f16, and the running maximum is only raised when a score
+// passes it by 2^8 (the factors cancel in o and sum alike; 2^15 fits f16).
+// Rows of q are scaled by a power of two into [1, 2) first: any fp32 magnitude
+// fits the f16 parts.
+//
+//   kv_prefix   tcgen05: the batch's q heads of one kv head are the rows of a
+//               [seqs * G, 128] x [128, prefix] product. Two softmax
+//               warpgroups work on two score tiles (128 rows x 128 tokens), so
+//               that one's exponentials run under the other's products: two
+//               row tiles that share each K / V tile, or, where one row tile
+//               is all there is, alternate token tiles. P stays in tensor
+//               memory (the A operand of P V, written over the scores).
+//               Bound by the tensor cores from about 256 rows a kv head, by
+//               HBM below.
+//   kv_own      a warp per piece: 16 tokens at a time through a private ring of
+//               cp.async stages, mma.sync m16n8k16 with the up to 8 q heads of
+//               a kv head as rows 0-7 (hi) and 8-15 (lo). Bound by HBM: the
+//               products of a step are 32 instructions for 8 KB, so what counts
+//               is that warps run on their own (no block barrier per tile, any
+//               length costs what it has), not the rate of the tensor pipe.
+//   kv_join     joins the pieces of every (sequence, q head) and turns the
+//               scores that kv_own kept into weights.
 #include "li_kv.cuh"
+#include "li_tc.cuh"
+
+#include <cuda.h>   // CUtensorMap and its enums; the encoder is fetched at run time
+
+#include <cstring>
+#include <mutex>
 
 LI_DEFINE_TU_STATUS(kvattn)
 
 namespace li {
 namespace {
 
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kPShift = 7.f;                 // probabilities carry 2^7
+constexpr float kMaxLag = 8.f;                 // the running maximum may lag by 2^8
+
+// ---- own part: pieces ------------------------------------------------------
+constexpr int kOwnTok = 16;                    // tokens per step
+constexpr int kOwnWarps = 8, kOwnThreads = kOwnWarps * kWarp;
+constexpr int kOwnStages = 3;
+constexpr int kOwnStageBytes = 2 * kOwnTok * kKvD * 2;      // K and V rows of a step: 8 KB
+constexpr size_t kOwnSmem = (size_t)kOwnWarps * kOwnStages * kOwnStageBytes;   // 192 KB
+constexpr int kOwnFlush = 16;                  // steps summed by mma before they join the record
+constexpr int kOwnMinSteps = 2;                // steps a warp takes at least, where there are enough
+constexpr int kScanMax = 2048;                 // entries of the length scan in shared memory
+
+// ---- prefix part -----------------------------------------------------------
+constexpr int kPreRows = 128, kPreTok = 128;
+constexpr int kPreThreads = 384;               // warps 0-3, 4-7: softmax; 8: TMA; 9, 10: MMA of buffer 0, 1
+constexpr int kPreRegsSoft = 208, kPreRegsRest = 88;        // 256 * 208 + 128 * 88 = 384 * 168
+constexpr uint32_t kPreSlotBytes = kPreTok * kKvD * 2;      // 128 tokens of K or V: 32 KB
+constexpr uint32_t kPreQBytes = 2 * kPreRows * kKvD * 2;    // a row tile's hi and lo: 64 KB
+constexpr int kPreSlots2 = 3, kPreSlots1 = 5;  // ring slots beside two / one row tiles of q
+constexpr int kPreFlush = 6;                   // token tiles summed in tensor memory before they join the record
+constexpr size_t kPreSmem = 1024 + 2 * kPreQBytes + kPreSlots2 * kPreSlotBytes + 256;
+static_assert(2 * kPreQBytes + kPreSlots2 * kPreSlotBytes == kPreQBytes + kPreSlots1 * kPreSlotBytes, "ring");
+
 struct KvAttnArgs {
     const float *q;
     int64_t q_stride;
-    const __half *k, *v, *kp, *vp;
+    const __half *k, *v;
     const int32_t *len;
-    int Hq, Hkv, G, max_ctx, n_prefix;
-    float scale, decay;
+    int B, Hq, Hkv, G, max_ctx;
+    float cscale;                      // |scale| log2(e)
+    float qsign;                       // sign of scale, applied to q
+    float decay;
     float *out, *weight;
+    // own part
+    int own_warps;                     // warps of the kv_own grid
+    int *base;                         // [B + 1] first step of every sequence (all kv heads), then the total
+    float2 *own_ml;                    // [pairs + own_warps][G]
+    float *own_o;                      // [pairs + own_warps][G][128]
+    float *score;                      // [B][Hq][max_ctx], log2 units (weight != nullptr)
+    bool after_prefix;
+    // prefix part
+    int n_prefix, rows, n_rt, per_group, n_grp, n_tt;   // rows = B G; row tiles; row tiles per group; groups; tiles
+    int pre_ctas, slots;
+    float2 *pre_ml;                    // [Hkv n_grp + pre_ctas][2][128]
+    float *pre_o;                      // [Hkv n_grp + pre_ctas][2][128][128]
+    // join
+    int row_ctas, wpr, w_chunks;       // blocks that join rows, warps per row, blocks per pair that write weights
 };
 
-// Block per (sequence, kv head), one q head after the other; a warp takes
-// every fourth token (a lane holds four dims), the warps merge at the end.
-__global__ void __launch_bounds__(128) kv_attn_kernel(KvAttnArgs a) {
-    __shared__ float wm[4], wl[4], wo[4][kKvD], gm[16], gl[16];
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ int own_len(const KvAttnArgs &a, int s) {
+    const int n = __ldcg(a.len + s);
+    return n < 0 || n > a.max_ctx ? 0 : n;
+}
+
+__device__ __forceinline__ int own_steps(int n) { return (n + kOwnTok - 1) / kOwnTok; }
+
+// Power of two 2^e with |x| / 2^e in [1, 2) (1 for 0, infinities and NaN).
+__device__ __forceinline__ float pow2_of(float x) {
+    const uint32_t e = (__float_as_uint(x) >> 23) & 255u;
+    return e == 0u || e == 255u ? 1.f : __uint_as_float(e << 23);
+}
+
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// hi keeps the top 11 bits of x (exact in f16), lo the rest.
+__device__ __forceinline__ float hi_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
+
+// A row's scale as 1 / 2^e: exact, and finite for every normal 2^e but 2^127.
+__device__ __forceinline__ float inv_pow2(float p) {
+    const uint32_t e = __float_as_uint(p) >> 23;
+    return __uint_as_float((e >= 254u ? 1u : 254u - e) << 23);
+}
+
+// ---------------------------------------------------------------------------
+// Pieces of the own part: the steps of all (sequence, kv head) pairs in order
+// (total T) are dealt to W warps in equal runs; warp w has [w T / W, (w+1) T / W).
+// The piece of pair p that warp w holds is record p + w: along the line of
+// steps either p or w grows from piece to piece, so no two share a record.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int own_active(int T, int warps) {
+    const int w = T / kOwnMinSteps;
+    return w < 1 ? 1 : w < warps ? w : warps;
+}
+__device__ __forceinline__ int run_begin(int w, int T, int W) { return (int)((int64_t)w * T / W); }
+__device__ __forceinline__ int run_of(int step, int T, int W) { return (int)((((int64_t)step + 1) * W - 1) / T); }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// NG groups of 8 q heads. In a warp, lane l holds q head l / 4 of each group
+// (scores of tokens 2 (l % 4), +1 of each 8; dims 2 (l % 4), +1 of each 8).
+template <int NG, bool SCORE>
+__global__ void __launch_bounds__(kOwnThreads, 1) kv_own_kernel(const __grid_constant__ KvAttnArgs a) {
+    extern __shared__ __align__(128) uint8_t own_smem[];
+    __shared__ int cum[kScanMax], wsum[kOwnWarps];
+    const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
+    // behind a prefix kernel, this one starts when that one has passed its own
+    // wait: everything either reads is in place; only the join needs both
+    if (!a.after_prefix) {
+        grid_dep_wait();
+        grid_dep_launch_dependents();
+    }
+    // Lengths: `per` neighbouring sequences an entry, a running sum of their steps.
+    const int per = (a.B + kScanMax - 1) / kScanMax, entries = (a.B + per - 1) / per;
+    int T = 0;
+    for (int e0 = 0; e0 < entries; e0 += kOwnThreads) {
+        const int e = e0 + tid;
+        int mine = 0;
+        for (int i = 0; i < per; ++i) {
+            const int s = e * per + i;
+            if (e < entries && s < a.B) {
+                const int n = __ldcg(a.len + s);
+                if (n < 0 || n > a.max_ctx) {
+                    if (blockIdx.x == 0) atomicExch(&g_device_error, LI_ERR_BAD_ARG);
+                } else {
+                    mine += own_steps(n);
+                }
+            }
+        }
+        mine *= a.Hkv;
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+        }
+        __syncthreads();
+        if (lane == 31) wsum[warp] = incl;
+        __syncthreads();
+        int off = T, all = 0;
+#pragma unroll
+        for (int w = 0; w < kOwnWarps; ++w) {
+            if (w < warp) off += wsum[w];
+            all += wsum[w];
+        }
+        if (e < entries) {
+            cum[e] = off + incl - mine;
+            if (blockIdx.x == 0) {
+                int at = off + incl - mine;
+                for (int i = 0; i < per && e * per + i < a.B; ++i) {
+                    a.base[e * per + i] = at;
+                    at += own_steps(own_len(a, e * per + i)) * a.Hkv;
+                }
+            }
+        }
+        T += all;
+    }
+    if (blockIdx.x == 0 && tid == 0) a.base[a.B] = T;
+    __syncthreads();
+
+    const int W = own_active(T, a.own_warps);
+    const int w = warp * gridDim.x + blockIdx.x;       // neighbouring pieces on different SMs
+    const int lo = w < W && T > 0 ? run_begin(w, T, W) : 0, hi = w < W && T > 0 ? run_begin(w + 1, T, W) : 0;
+    const int n_steps = hi - lo;
+    if (n_steps > 0) {
+        // a cursor: sequence, kv head, step within the pair, and the sequence's length
+        struct Cursor { int s, j, t, n; };
+        Cursor ld;
+        {
+            int e = 0, end = entries;                  // the last entry that starts at or before lo
+            while (end - e > 1) {
+                const int mid = (e + end) / 2;
+                if (cum[mid] <= lo) e = mid; else end = mid;
+            }
+            int at = cum[e], s = e * per, n = own_len(a, s);
+            while (at + own_steps(n) * a.Hkv <= lo) {
+                at += own_steps(n) * a.Hkv;
+                n = own_len(a, ++s);
+            }
+            const int in = lo - at, st = own_steps(n);
+            ld.s = s; ld.n = n; ld.j = in / st; ld.t = in - ld.j * st;
+        }
+        auto next = [&](Cursor &c) {
+            if (++c.t < own_steps(c.n)) return;
+            c.t = 0;
+            if (++c.j < a.Hkv) return;
+            c.j = 0;
+            do {
+                if (++c.s >= a.B) { c.n = 0; return; }
+                c.n = own_len(a, c.s);
+            } while (c.n == 0);
+        };
+        Cursor cu = ld;
+        const uint32_t ring = smem_addr(own_smem) + (uint32_t)warp * kOwnStages * kOwnStageBytes;
+        const size_t row = (size_t)a.Hkv * kKvD;
+        const int lr = lane >> 4, lc = lane & 15;      // this lane's row (of two) and 16-byte piece in a copy
+        auto issue = [&](const Cursor &c, int stage) {
+            const size_t at = ((size_t)c.s * a.max_ctx + (size_t)c.t * kOwnTok) * row + (size_t)c.j * kKvD + 8 * lc;
+            const int left = c.n - c.t * kOwnTok;
+            const uint32_t dst = ring + (uint32_t)stage * kOwnStageBytes;
+#pragma unroll
+            for (int i = 0; i < kOwnTok / 2; ++i) {
+                const int r = 2 * i + lr;
+                const bool ok = r < left;              // past the length: zeros, whatever the slot holds
+                const size_t src = at + (ok ? (size_t)r * row : 0);
+                const uint32_t d = dst + (uint32_t)(r * 256 + ((lc ^ (r & 7)) << 4));
+                cp_async16(d, a.k + src, ok);
+                cp_async16(d + kOwnTok * 256, a.v + src, ok);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < kOwnStages - 1; ++i) {
+            if (i < n_steps) {
+                issue(ld, i);
+                next(ld);
+            }
+            cp_async_commit();
+        }
+        uint32_t qf[NG][8][4];
+        float o[NG][16][4], m[NG], l[NG], c2[NG], m_rec[NG];
+        bool fresh = true;
+        int since = 0;                                 // steps in o that are not in the record
+        const int g = lane >> 2, tq = lane & 3;
+        const int kc = lane >> 3, kr = lane & 7;       // ldmatrix: matrix and row this lane addresses
+        int stage = 0, ld_stage = kOwnStages - 1;
+        for (int i = 0; i < n_steps; ++i) {
+            cp_async_wait<kOwnStages - 2>();
+            __syncwarp();                              // this step has landed; the last one's stage is free
+            if (i + kOwnStages - 1 < n_steps) {
+                issue(ld, ld_stage);
+                next(ld);
+            }
+            cp_async_commit();
+            ld_stage = ld_stage + 1 == kOwnStages ? 0 : ld_stage + 1;
+            if (fresh) {                               // a new pair: its q heads, scaled and split
+#pragma unroll
+                for (int e = 0; e < NG; ++e) {
+                    const int h = 8 * e + g;
+                    const float *qs = a.q + cu.s * a.q_stride + (size_t)(cu.j * a.G + h) * kKvD + 2 * tq;
+                    float2 x[16];
+                    float mx = 0.f;
+#pragma unroll
+                    for (int kk = 0; kk < 16; ++kk) {
+                        x[kk] = h < a.G ? __ldcg(reinterpret_cast<const float2 *>(qs + 8 * kk)) : make_float2(0.f, 0.f);
+                        mx = fmaxf(mx, fmaxf(fabsf(x[kk].x), fabsf(x[kk].y)));
+                    }
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    const float p2 = pow2_of(mx), inv = inv_pow2(p2) * a.qsign;
+                    c2[e] = a.cscale * p2;
+#pragma unroll
+                    for (int kk = 0; kk < 16; ++kk) {
+                        const float y0 = x[kk].x * inv, y1 = x[kk].y * inv, h0 = hi_part(y0), h1 = hi_part(y1);
+                        qf[e][kk >> 1][(kk & 1) * 2] = pack_h2(h0, h1);
+                        qf[e][kk >> 1][(kk & 1) * 2 + 1] = pack_h2(y0 - h0, y1 - h1);
+                    }
+                    m[e] = m_rec[e] = -INFINITY;
+                    l[e] = 0.f;
+#pragma unroll
+                    for (int nt = 0; nt < 16; ++nt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[e][nt][r] = 0.f;
+                }
+                fresh = false;
+                since = 0;
+            }
+            const uint32_t kb = ring + (uint32_t)stage * kOwnStageBytes, vb = kb + kOwnTok * 256;
+            stage = stage + 1 == kOwnStages ? 0 : stage + 1;
+            // scores of 16 tokens: two 8-token tiles, 128 dims in eight k-steps
+            float sc[NG][2][4];
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+#pragma unroll
+                for (int e = 0; e < NG; ++e)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sc[e][nt][r] = 0.f;
+                const uint32_t tok = kb + (uint32_t)(8 * nt + kr) * 256;
+#pragma unroll
+                for (int kp = 0; kp < 4; ++kp) {
+                    uint32_t b[4];
+                    ldsm4(tok + (uint32_t)(((4 * kp + kc) ^ kr) << 4), b);
+#pragma unroll
+                    for (int e = 0; e < NG; ++e) {
+                        mma_f16(sc[e][nt], qf[e][2 * kp], b[0], b[1]);
+                        mma_f16(sc[e][nt], qf[e][2 * kp + 1], b[2], b[3]);
+                    }
+                }
+            }
+            const int t0 = cu.t * kOwnTok, left = cu.n - t0;
+            uint32_t pf[NG][4];
+#pragma unroll
+            for (int e = 0; e < NG; ++e) {
+                float s2[4];
+                float mx = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int nt = x >> 1, r = x & 1, tok = 8 * nt + 2 * tq + r;
+                    s2[x] = (sc[e][nt][r] + sc[e][nt][2 + r]) * c2[e];
+                    if (SCORE && 8 * e + g < a.G && tok < left)
+                        a.score[((size_t)cu.s * a.Hq + (size_t)cu.j * a.G + 8 * e + g) * a.max_ctx + t0 + tok] = s2[x];
+                    if (tok >= left) s2[x] = -INFINITY;
+                    mx = fmaxf(mx, s2[x]);
+                }
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const bool grow = mx > m[e] + kMaxLag;     // also the first step: m = -inf
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float f = !grow ? 1.f : m[e] == -INFINITY ? 0.f : ex2(m[e] - mx);
+                    if (grow) m[e] = mx;
+                    l[e] *= f;
+#pragma unroll
+                    for (int nt = 0; nt < 16; ++nt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[e][nt][r] *= f;
+                }
+                float p[4], ph[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    p[x] = ex2(s2[x] - m[e] + kPShift);
+                    l[e] += p[x];
+                    ph[x] = hi_part(p[x]);
+                }
+                pf[e][0] = pack_h2(ph[0], ph[1]);
+                pf[e][1] = pack_h2(p[0] - ph[0], p[1] - ph[1]);
+                pf[e][2] = pack_h2(ph[2], ph[3]);
+                pf[e][3] = pack_h2(p[2] - ph[2], p[3] - ph[3]);
+            }
+            // o += P V: 16 tokens, 128 dims in 16 tiles
+            const uint32_t vt = vb + (uint32_t)(((kc & 1) * 8 + kr) * 256);
+#pragma unroll
+            for (int dp = 0; dp < 8; ++dp) {
+                uint32_t b[4];
+                ldsm4_t(vt + (uint32_t)(((2 * dp + (kc >> 1)) ^ kr) << 4), b);
+#pragma unroll
+                for (int e = 0; e < NG; ++e) {
+                    mma_f16(o[e][2 * dp], pf[e], b[0], b[1]);
+                    mma_f16(o[e][2 * dp + 1], pf[e], b[2], b[3]);
+                }
+            }
+            const int ps = cu.s, pj = cu.j;
+            next(cu);
+            fresh = cu.s != ps || cu.j != pj;
+            const bool last = fresh || i + 1 == n_steps;
+            if (last || ++since == kOwnFlush) {
+                // o joins the record, whose values have the factor 2^(m_rec)
+                const size_t rec = (size_t)ps * a.Hkv + pj + w;
+                since = 0;
+#pragma unroll
+                for (int e = 0; e < NG; ++e) {
+                    float sum = l[e] + __shfl_xor_sync(0xffffffffu, l[e], 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    const int h = 8 * e + g;
+                    if (h < a.G) {
+                        if (last && tq == 0) a.own_ml[rec * a.G + h] = make_float2(m[e] - kPShift, sum);
+                        float *d = a.own_o + (rec * a.G + h) * kKvD + 2 * tq;
+                        const bool again = m_rec[e] != -INFINITY;
+                        const float fr = again ? ex2(m_rec[e] - m[e]) : 0.f;
+#pragma unroll
+                        for (int nt = 0; nt < 16; ++nt) {
+                            float2 x = make_float2(o[e][nt][0] + o[e][nt][2], o[e][nt][1] + o[e][nt][3]);
+                            if (again) {
+                                const float2 old = *reinterpret_cast<const float2 *>(d + 8 * nt);
+                                x.x = fmaf(old.x, fr, x.x);
+                                x.y = fmaf(old.y, fr, x.y);
+                            }
+                            *reinterpret_cast<float2 *>(d + 8 * nt) = x;
+                        }
+                    }
+                    m_rec[e] = m[e];
+#pragma unroll
+                    for (int nt = 0; nt < 16; ++nt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[e][nt][r] = 0.f;
+                }
+            }
+        }
+        cp_async_wait<0>();
+    }
+    if (a.after_prefix) {
+        grid_dep_launch_dependents();
+        grid_dep_wait();       // the join follows both kernels
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Pieces of the prefix part. Row tiles of one kv head go in groups of one or
+// two (per_group); a group's token tile costs its number of row tiles. The
+// line of all costs (kv heads, then groups) is dealt to the blocks in equal
+// runs, a block's boundary rounded up to a whole token tile. The piece of
+// group p that block c holds is record p + c, as above.
+// ---------------------------------------------------------------------------
+struct Group { int j, rt, nt, base; };         // kv head, first row tile, row tiles, place on the line
+
+__device__ __forceinline__ Group group_at(const KvAttnArgs &a, int p) {
+    Group g;
+    g.j = p / a.n_grp;
+    g.rt = (p - g.j * a.n_grp) * a.per_group;
+    g.nt = a.n_rt - g.rt < a.per_group ? a.n_rt - g.rt : a.per_group;
+    g.base = (g.j * a.n_rt + g.rt) * a.n_tt;
+    return g;
+}
+// token tiles [t0, t1) of group g in the run [lo, hi)
+__device__ __forceinline__ void tiles_of(const KvAttnArgs &a, const Group &g, int lo, int hi, int &t0, int &t1) {
+    t0 = lo <= g.base ? 0 : (lo - g.base + g.nt - 1) / g.nt;
+    t1 = hi <= g.base ? 0 : (hi - g.base + g.nt - 1) / g.nt;
+    if (t1 > a.n_tt) t1 = a.n_tt;
+}
+
+__device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *map, int x, int y, int z,
+                                            uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_addr(smem_dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+        : "memory");
+}
+
+// A bounded wait that also gives up once another warp has.
+__device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (!mbar_wait(bar, parity)) {
+        *abort_flag = 1;
+        return false;
+    }
+    return true;
+}
+
+// Named barrier 1 over the eight softmax warps, returning whether any passed v.
+__device__ __forceinline__ bool softmax_bar_any(bool v) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred pi, po;\n\tsetp.ne.u32 pi, %1, 0;\n\t"
+                 "bar.red.or.pred po, 1, 256, pi;\n\tselp.u32 %0, 1, 0, po;\n\t}"
+                 : "=r"(r) : "r"((uint32_t)v) : "memory");
+    return r != 0;
+}
+
+// Order in which the K and V tiles of a piece of n token tiles go through the
+// ring: place i = 0 .. 2n-1 holds K or V of token tile t. With two row tiles
+// (nt 2) both buffers use every tile: K0 V0 K1 V1 ...; with one, buffer b takes
+// the tiles t % 2 == b: K0 K1 V0 K2 V1 K3 V2 ...
+__device__ __forceinline__ void ring_place(int i, int n, int nt, int &t, bool &is_v) {
+    if (nt == 2) {
+        t = i >> 1;
+        is_v = i & 1;
+    } else if (i == 2 * n - 1) {
+        t = n - 1;
+        is_v = true;
+    } else {
+        is_v = i > 0 && !(i & 1);
+        t = is_v ? (i - 2) >> 1 : (i + 1) >> 1;
+    }
+}
+
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// Adds to global memory without waiting. A record's words are only ever
+// touched by one thread, so its sums have one order.
+__device__ __forceinline__ void red_add4(float4 *p, float a, float b, float c, float d) {
+    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(a), "f"(b), "f"(c), "f"(d)
+                 : "memory");
+}
+__device__ __forceinline__ void red_add2(float2 *p, float a, float b) {
+    asm volatile("red.relaxed.gpu.global.add.v2.f32 [%0], {%1, %2};" ::"l"(p), "f"(a), "f"(b) : "memory");
+}
+
+__global__ void __launch_bounds__(kPreThreads, 1)
+kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const __grid_constant__ KvAttnArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    uint8_t *qbuf = smem;                                          // [row tile][hi, lo][2 blocks of 64 dims][128 rows]
+    uint8_t *ring = smem + (size_t)a.per_group * kPreQBytes;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + 2 * kPreQBytes + kPreSlots2 * kPreSlotBytes);
+    uint64_t *full = bars, *empty = full + kPreSlots1, *q_full = empty + kPreSlots1, *s_full = q_full + 1,
+             *p_full = s_full + 2, *o_full = p_full + 2, *fin = o_full + 2;
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(fin + 2);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
+    const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
+    const int slots = a.slots;
+    if (tid == 0) {
+        for (int i = 0; i < slots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 2); }
+        mbar_init(q_full, 8);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_full[i], 1);
+            mbar_init(&fin[i], 1);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 8) tmem_alloc(tmem_holder, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_holder;                            // scores / P of buffers 0, 1, then o of 0, 1
     grid_dep_wait();
     grid_dep_launch_dependents();
-    const int s = blockIdx.x / a.Hkv, j = blockIdx.x % a.Hkv;
-    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
-    int n = a.len[s];
-    if (n < 0 || n > a.max_ctx) {
-        if (threadIdx.x == 0) atomicExch(&g_device_error, LI_ERR_BAD_ARG);
-        n = 0;
+
+    const int cost = a.Hkv * a.n_rt * a.n_tt, c = blockIdx.x;
+    const int lo = (int)((int64_t)cost * c / a.pre_ctas), hi = (int)((int64_t)cost * (c + 1) / a.pre_ctas);
+    int p0;                                                        // the group that lo falls into
+    {
+        const int per_j = a.n_rt * a.n_tt, j = lo / per_j;
+        p0 = j * a.n_grp + (lo - j * per_j) / (a.per_group * a.n_tt);
     }
-    const size_t row = (size_t)a.Hkv * kKvD, own0 = ((size_t)s * a.max_ctx * a.Hkv + j) * kKvD;
-    auto at = [&](const __half *pre, const __half *own, int t) {
-        const __half *p = t < a.n_prefix ? pre + (size_t)t * row + (size_t)j * kKvD
-                                         : own + own0 + (size_t)(t - a.n_prefix) * row;
-        const uint2 u = *reinterpret_cast<const uint2 *>(p + 4 * lane);
-        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&u.x));
-        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
-        return make_float4(x.x, x.y, y.x, y.y);
-    };
-    auto score = [&](const float4 q, int t) {
-        const float4 k = at(a.kp, a.k, t);
-        return warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w) * a.scale;
-    };
-    const int total = a.n_prefix + n;
-    for (int g = 0; g < a.G; ++g) {
-        const int h = j * a.G + g;
-        const float4 q = *reinterpret_cast<const float4 *>(a.q + s * a.q_stride + (size_t)h * kKvD + 4 * lane);
+    const int p_end = a.Hkv * a.n_grp;
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsRest));
+        if (warp == 8 && lane == 0) {
+            // ---------------- producer ----------------
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&tmK) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&tmV) : "memory");
+            int slot = 0, used = 0;
+            uint32_t par = 1;                                      // of the slot's previous release
+            bool ok = true;
+            for (int p = p0; ok && p < p_end; ++p) {
+                const Group g = group_at(a, p);
+                if (g.base >= hi) break;
+                int t0, t1;
+                tiles_of(a, g, lo, hi, t0, t1);
+                const int n = t1 - t0;
+                for (int i = 0; i < 2 * n; ++i) {
+                    int t;
+                    bool is_v;
+                    ring_place(i, n, g.nt, t, is_v);
+                    if (used >= slots && !(ok = wait_or_abort(&empty[slot], par, abort_flag))) break;
+                    mbar_arrive_expect_tx(&full[slot], kPreSlotBytes);
+                    uint8_t *dst = ring + (size_t)slot * kPreSlotBytes;
+                    const CUtensorMap *map = is_v ? &tmV : &tmK;
+                    const int z = (t0 + t) * kPreTok;
+                    tma_load_3d(dst, map, 0, g.j, z, &full[slot]);
+                    tma_load_3d(dst + kPreSlotBytes / 2, map, 64, g.j, z, &full[slot]);
+                    ++used;
+                    if (++slot == slots) { slot = 0; par ^= 1u; }
+                }
+            }
+            // every copy issued has landed before the block ends
+            for (int k = used < slots ? 0 : used - slots; k < used; ++k)
+                mbar_wait(&full[k % slots], (uint32_t)((k / slots) & 1));
+        } else if ((warp == 9 || warp == 10) && lane == 0) {
+            // ---------------- MMA issuer of buffer b ----------------
+            // The thread stands still while an MMA is taken, so what it does
+            // between them adds to the tensor pipe's time; the two issuers
+            // cover for each other, and descriptors advance by constants.
+            const int b = warp - 9;
+            const uint32_t id_s = idesc_kf16(128, kPreTok, false);
+            const uint32_t id_o = idesc_kf16(128, kKvD, false) | kIdescBMajorMN;
+            const uint64_t k0 = sw128_desc(smem_addr(ring)), v0 = sw128_mn_desc(smem_addr(ring), kPreSlotBytes / 2);
+            const uint32_t ts = tmem + 128u * b, to = tmem + 256u + 128u * b;
+            int slot = 0;
+            uint32_t par = 0, pq = 0, pp = 0;                      // phases of the slot, q_full, p_full
+            bool ok = true;
+            for (int p = p0; ok && p < p_end; ++p) {
+                const Group g = group_at(a, p);
+                if (g.base >= hi) break;
+                int t0, t1;
+                tiles_of(a, g, lo, hi, t0, t1);
+                const int n = t1 - t0;
+                if (n <= 0) continue;
+                if (!(ok = wait_or_abort(q_full, pq, abort_flag))) break;
+                pq ^= 1u;
+                const uint64_t q_hi = sw128_desc(smem_addr(qbuf) + (g.nt == 2 ? (uint32_t)b * kPreQBytes : 0u));
+                const int last = g.nt == 2 || ((n - 1) & 1) == b ? n - 1 : n - 2;      // this buffer's last tile
+                int unit = 0;
+                for (int i = 0; i < 2 * n; ++i) {
+                    int t;
+                    bool is_v;
+                    ring_place(i, n, g.nt, t, is_v);
+                    const bool mine = g.nt == 2 || (t & 1) == b;
+                    if (mine && is_v) {
+                        if (!(ok = wait_or_abort(&p_full[b], pp, abort_flag))) break;
+                        pp ^= 1u;
+                    }
+                    if (!(ok = wait_or_abort(&full[slot], par, abort_flag))) break;
+                    if (!mine) {
+                        mbar_arrive(&empty[slot]);
+                    } else if (!is_v) {
+                        // S = Q K^T; lo first, so that only the hi products add to a sum of full size (the
+                        // tensor cores' sums round towards zero, once per instruction)
+                        tc_fence_after();
+                        const uint64_t kd = k0 + (uint64_t)(slot * (kPreSlotBytes >> 4));
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) {
+                            const uint32_t at = 1024u * ((x & 7) >> 2) + 2u * (x & 3);
+                            umma_f16(ts, q_hi + (x < 8 ? 2048u : 0u) + at, kd + at, id_s, x ? 1u : 0u);
+                        }
+                        umma_commit(&s_full[b]);
+                        umma_commit(&empty[slot]);
+                    } else {
+                        tc_fence_after();
+                        const uint64_t vd = v0 + (uint64_t)(slot * (kPreSlotBytes >> 4));
+                        const uint32_t again = unit % kPreFlush ? 1u : 0u;
+#pragma unroll
+                        for (int x = 0; x < 16; ++x)
+                            umma_f16_ta(to, ts + (x < 8 ? 64u : 0u) + 8u * (x & 7), vd + 128u * (x & 7), id_o,
+                                        x ? 1u : again);
+                        if (t == last) umma_commit(&o_full[b]);
+                        umma_commit(&empty[slot]);
+                        ++unit;
+                    }
+                    if (++slot == slots) { slot = 0; par ^= 1u; }
+                }
+                // a piece of one tile leaves buffer 1 nothing to do; o_full counts pieces all the same, so that no
+                // issuer falls a piece behind
+                if (last < 0) mbar_arrive(&o_full[b]);
+            }
+            umma_commit(&fin[b]);
+            mbar_wait(&fin[b], 0u);
+        }
+    } else {
+        // ---------------- softmax: a thread per row of its score buffer ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPreRegsSoft));
+        const int b = warp >> 2, r = tid & 127;
+        const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        const uint32_t sb = lane_base + 128u * b, ob = lane_base + 256u + 128u * b;
+        uint32_t ps = 0, po = 0;                                   // phases of s_full, o_full
+        bool stop = false;
+        for (int p = p0; !stop && p < p_end; ++p) {
+            const Group g = group_at(a, p);
+            if (g.base >= hi) break;
+            int t0, t1;
+            tiles_of(a, g, lo, hi, t0, t1);
+            const int n = t1 - t0;
+            if (n <= 0) continue;
+            // this row's q: scaled, split and stored as the operand's rows
+            const int row = (g.rt + (g.nt == 2 ? b : 0)) * kPreRows + r;
+            const bool live = row < a.rows;
+            float c2;
+            {
+                const int s = live ? row / a.G : 0, h = live ? g.j * a.G + row - s * a.G : 0;
+                const float4 *qs = reinterpret_cast<const float4 *>(a.q + s * a.q_stride + (size_t)h * kKvD);
+                float4 x[32];
+                float mx = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    x[i] = live ? __ldcg(qs + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+                }
+                const float p2 = pow2_of(mx), inv = inv_pow2(p2) * a.qsign;
+                c2 = fmaxf(a.cscale * p2, 1.17549435e-38f);        // not 0: a masked score is -inf c2
+                if (g.nt == 2 || b == 0) {
+                    uint8_t *qd = qbuf + (g.nt == 2 ? (size_t)b * kPreQBytes : 0);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float y[8] = {x[2 * i].x * inv, x[2 * i].y * inv, x[2 * i].z * inv, x[2 * i].w * inv,
+                                            x[2 * i + 1].x * inv, x[2 * i + 1].y * inv, x[2 * i + 1].z * inv,
+                                            x[2 * i + 1].w * inv};
+                        uint32_t hw[4], lw[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float h0 = hi_part(y[2 * e]), h1 = hi_part(y[2 * e + 1]);
+                            hw[e] = pack_h2(h0, h1);
+                            lw[e] = pack_h2(y[2 * e] - h0, y[2 * e + 1] - h1);
+                        }
+                        const uint32_t off = (uint32_t)(i >> 3) * 16384u + sw128_off(r, i & 7);
+                        *reinterpret_cast<uint4 *>(qd + off) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                        *reinterpret_cast<uint4 *>(qd + 32768 + off) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                    }
+                }
+            }
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+            float m = -INFINITY, l = 0.f, m_rec = -INFINITY;
+            bool ok = true;
+            const size_t rec = ((size_t)(p + c) * 2 + b) * kPreRows + r;
+            float4 *d = reinterpret_cast<float4 *>(a.pre_o + rec * kKvD);
+            // o in tensor memory joins this row of the record, whose values have the factor 2^(m_rec)
+            auto flush = [&]() {
+                const float fr = m_rec == -INFINITY ? 0.f : ex2(m_rec - m);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t ov[32];
+                    tmem_ld32_nowait(ob + 32u * x, ov);
+                    tmem_wait_ld();
+                    if (!live) continue;
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) {
+                        float4 w = make_float4(__uint_as_float(ov[4 * y]), __uint_as_float(ov[4 * y + 1]),
+                                               __uint_as_float(ov[4 * y + 2]), __uint_as_float(ov[4 * y + 3]));
+                        if (m_rec == m) {
+                            red_add4(d + 8 * x + y, w.x, w.y, w.z, w.w);
+                            continue;
+                        }
+                        if (m_rec != -INFINITY) {
+                            const float4 old = __ldcg(d + 8 * x + y);
+                            w.x = fmaf(old.x, fr, w.x); w.y = fmaf(old.y, fr, w.y);
+                            w.z = fmaf(old.z, fr, w.z); w.w = fmaf(old.w, fr, w.w);
+                        }
+                        __stcg(d + 8 * x + y, w);
+                    }
+                }
+                m_rec = m;
+            };
+            int unit = 0;
+            // this buffer's token tiles: every one (nt 2), or every second one
+            const int first = g.nt == 2 ? 0 : b, step = g.nt == 2 ? 1 : 2;
+            for (int i = first; i < n; i += step, ++unit) {
+                ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[b], ps, abort_flag));
+                if (!ok) break;
+                ps ^= 1u;
+                tc_fence_after();
+                // P V of this buffer's last tile is complete: these scores were issued after it
+                if (unit > 0 && unit % kPreFlush == 0) flush();
+                uint32_t v[4][32];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) tmem_ld32_nowait(sb + 32u * x, v[x]);
+                tmem_wait_ld();
+                const int left = a.n_prefix - (t0 + i) * kPreTok;
+                if (left < kPreTok) {
+#pragma unroll
+                    for (int x = 0; x < 128; ++x)
+                        if (x >= left) v[x >> 5][x & 31] = 0xff800000u;            // -inf
+                }
+                float m8[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    m8[x] = fmaxf(__uint_as_float(v[0][x]), fmaxf(__uint_as_float(v[0][8 + x]),
+                                                                  __uint_as_float(v[0][16 + x])));
+#pragma unroll
+                for (int y = 24; y < 120; y += 16)
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const int e = y + x, f = y + 8 + x;
+                        m8[x] = fmaxf(m8[x], fmaxf(__uint_as_float(v[e >> 5][e & 31]), __uint_as_float(v[f >> 5][f & 31])));
+                    }
+#pragma unroll
+                for (int x = 0; x < 8; ++x) m8[x] = fmaxf(m8[x], __uint_as_float(v[3][24 + x]));
+                const float mx = c2 * fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
+                                            fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
+                const bool grow = mx > m + kMaxLag;
+                const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2(m - mx);
+                if (grow) m = mx;
+                l *= f;
+                if (unit % kPreFlush && __any_sync(0xffffffffu, grow)) {
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t ov[32];
+                        tmem_ld32_nowait(ob + 32u * x, ov);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int y = 0; y < 32; ++y) ov[y] = __float_as_uint(__uint_as_float(ov[y]) * f);
+                        tmem_st32(ob + 32u * x, ov);
+                    }
+                }
+                const uint64_t cc = pack2(c2, c2), off = pack2(kPShift - m, kPShift - m), minus = pack2(-1.f, -1.f);
+                uint64_t ls[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint32_t hw[32], lw[32];
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) {
+                        const int e = 64 * hf + 2 * x;
+                        float p0, p1, d0, d1;
+                        unpack2(fma2(pack2(__uint_as_float(v[e >> 5][e & 31]), __uint_as_float(v[e >> 5][(e & 31) + 1])),
+                                     cc, off), p0, p1);
+                        p0 = ex2(p0);
+                        p1 = ex2(p1);
+                        const uint64_t pp = pack2(p0, p1);
+                        ls[x & 3] = add2(ls[x & 3], pp);
+                        const float h0 = hi_part(p0), h1 = hi_part(p1);
+                        hw[x] = pack_h2(h0, h1);
+                        unpack2(fma2(pack2(h0, h1), minus, pp), d0, d1);
+                        lw[x] = pack_h2(d0, d1);
+                    }
+                    tmem_st32(sb + 32u * hf, hw);
+                    tmem_st32(sb + 64u + 32u * hf, lw);
+                }
+                {
+                    float l0, l1;
+                    unpack2(add2(add2(ls[0], ls[1]), add2(ls[2], ls[3])), l0, l1);
+                    l += l0 + l1;
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[b]);
+            }
+            if (ok) {
+                ok = __all_sync(0xffffffffu, wait_or_abort(&o_full[b], po, abort_flag));
+                po ^= 1u;
+                if (ok && first < n) {
+                    tc_fence_after();
+                    flush();
+                    if (live) a.pre_ml[rec] = make_float2(m - kPShift, l);
+                    tc_fence_before();
+                }
+            }
+            // both buffers are done with q before the next piece's is written
+            stop = softmax_bar_any(!ok);
+        }
+    }
+    if (*abort_flag && tid == 0) atomicExch(&g_device_error, LI_ERR_TIMEOUT);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The join. Record i of row (s, h): the prefix's pieces first, then the own
+// part's; returns its place, or -1 for a piece that holds no token.
+// ---------------------------------------------------------------------------
+struct RowPieces {
+    int n_pre, n_own;
+    // prefix
+    Group g;
+    int p, c0, streams, stream0, prow;
+    // own
+    int rec0;
+};
+
+__device__ __forceinline__ RowPieces pieces_of(const KvAttnArgs &a, int s, int h) {
+    RowPieces x;
+    const int j = h / a.G, gq = h - j * a.G;
+    x.n_pre = x.n_own = 0;
+    if (a.n_prefix > 0) {
+        const int row = s * a.G + gq, rt = row / kPreRows;
+        x.prow = row - rt * kPreRows;
+        x.p = j * a.n_grp + rt / a.per_group;
+        x.g = group_at(a, x.p);
+        const int cost = a.Hkv * a.n_rt * a.n_tt;
+        x.c0 = run_of(x.g.base, cost, a.pre_ctas);
+        const int c1 = run_of(x.g.base + x.g.nt * a.n_tt - 1, cost, a.pre_ctas);
+        x.streams = x.g.nt == 2 ? 1 : 2;
+        x.stream0 = x.g.nt == 2 ? rt - x.g.rt : 0;
+        x.n_pre = (c1 - x.c0 + 1) * x.streams;
+    }
+    const int n = own_len(a, s);
+    if (n > 0) {
+        const int T = __ldcg(a.base + a.B), W = own_active(T, a.own_warps), st = own_steps(n);
+        const int b0 = __ldcg(a.base + s) + j * st;
+        const int w0 = run_of(b0, T, W), w1 = run_of(b0 + st - 1, T, W);
+        x.rec0 = s * a.Hkv + j + w0;
+        x.n_own = w1 - w0 + 1;
+    }
+    return x;
+}
+
+// (max, sum) of record i; its o in *o. (-inf, 0) for an empty one.
+__device__ __forceinline__ float2 piece_ml(const KvAttnArgs &a, const RowPieces &x, int gq, int i, const float **o) {
+    if (i < x.n_pre) {
+        const int c = x.c0 + i / x.streams, w = x.stream0 + i % x.streams;
+        const int cost = a.Hkv * a.n_rt * a.n_tt;
+        int t0, t1;
+        tiles_of(a, x.g, (int)((int64_t)cost * c / a.pre_ctas), (int)((int64_t)cost * (c + 1) / a.pre_ctas), t0, t1);
+        if (t1 - t0 <= (x.streams == 2 ? w : 0)) {
+            *o = nullptr;
+            return make_float2(-INFINITY, 0.f);
+        }
+        const size_t rec = ((size_t)(x.p + c) * 2 + w) * kPreRows + x.prow;
+        *o = a.pre_o + rec * kKvD;
+        return __ldcg(a.pre_ml + rec);
+    }
+    const size_t rec = (size_t)(x.rec0 + i - x.n_pre) * a.G + gq;
+    *o = a.own_o + rec * kKvD;
+    return __ldcg(a.own_ml + rec);
+}
+
+constexpr int kJoinWarps = 8;
+
+__global__ void __launch_bounds__(kJoinWarps * kWarp) kv_join_kernel(const __grid_constant__ KvAttnArgs a) {
+    __shared__ float red_m[kJoinWarps], red_l[kJoinWarps];
+    __shared__ __align__(16) float red_o[kJoinWarps][kKvD];
+    __shared__ float gm[16], gi[16];
+    grid_dep_wait();
+    grid_dep_launch_dependents();
+    const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
+    if ((int)blockIdx.x < a.row_ctas) {
+        // a row (s, h) on wpr neighbouring warps, each over its share of the records
+        const int per = kJoinWarps / a.wpr, sub = warp % a.wpr;
+        const int64_t rowi = (int64_t)blockIdx.x * per + warp / a.wpr;
+        const bool on = rowi < (int64_t)a.B * a.Hq;
         float m = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int t = warp; t < total; t += 4) {
-            const float sc = score(q, t), mn = fmaxf(m, sc);
-            const float al = m == -INFINITY ? 0.f : expf(m - mn), p = expf(sc - mn);
-            const float4 v = at(a.vp, a.v, t);
-            o.x = o.x * al + p * v.x; o.y = o.y * al + p * v.y; o.z = o.z * al + p * v.z; o.w = o.w * al + p * v.w;
-            l = l * al + p;
-            m = mn;
+        const int s = on ? (int)(rowi / a.Hq) : 0, h = on ? (int)(rowi - (int64_t)s * a.Hq) : 0;
+        if (on) {
+            const RowPieces x = pieces_of(a, s, h);
+            const int n = x.n_pre + x.n_own, gq = h % a.G;
+            for (int i0 = sub * kWarp; i0 < n; i0 += a.wpr * kWarp) {
+                const float *src = nullptr;
+                const float2 ml = i0 + lane < n ? piece_ml(a, x, gq, i0 + lane, &src) : make_float2(-INFINITY, 0.f);
+                float mx = ml.x;
+#pragma unroll
+                for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+                mx = fmaxf(mx, m);
+                const float keep = m == -INFINITY ? 0.f : ex2(m - mx), f = src ? ex2(ml.x - mx) : 0.f;
+                m = mx;
+                l = l * keep + warp_sum(f * ml.y);
+                o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
+                const int cnt = min(kWarp, n - i0);
+#pragma unroll 4
+                for (int k = 0; k < cnt; ++k) {
+                    const float fk = __shfl_sync(0xffffffffu, f, k);
+                    const float *ok = reinterpret_cast<const float *>(
+                        __shfl_sync(0xffffffffu, (unsigned long long)reinterpret_cast<uintptr_t>(src), k));
+                    if (ok) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(ok) + lane);
+                        o.x = fmaf(fk, v.x, o.x); o.y = fmaf(fk, v.y, o.y);
+                        o.z = fmaf(fk, v.z, o.z); o.w = fmaf(fk, v.w, o.w);
+                    }
+                }
+            }
         }
-        __syncthreads();
-        *reinterpret_cast<float4 *>(&wo[warp][4 * lane]) = o;
-        if (lane == 0) { wm[warp] = m; wl[warp] = l; }
-        __syncthreads();
-        float M = -INFINITY, L = 0.f, O = 0.f;
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, wm[w]);
-        for (int w = 0; w < 4; ++w) {
-            const float f = wm[w] == -INFINITY ? 0.f : expf(wm[w] - M);
-            L += f * wl[w];
-            O += f * wo[w][threadIdx.x];
+        if (a.wpr > 1) {
+            if (lane == 0) { red_m[warp] = m; red_l[warp] = l; }
+            reinterpret_cast<float4 *>(red_o[warp])[lane] = o;
+            __syncthreads();
+            if (sub == 0) {
+                float M = m;
+                for (int k = 1; k < a.wpr; ++k) M = fmaxf(M, red_m[warp + k]);
+                const float f0 = m == -INFINITY ? 0.f : ex2(m - M);
+                l *= f0;
+                o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+                for (int k = 1; k < a.wpr; ++k) {
+                    const float f = red_m[warp + k] == -INFINITY ? 0.f : ex2(red_m[warp + k] - M);
+                    const float4 v = reinterpret_cast<const float4 *>(red_o[warp + k])[lane];
+                    l = fmaf(f, red_l[warp + k], l);
+                    o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+                }
+            }
         }
-        a.out[((size_t)s * a.Hq + h) * kKvD + threadIdx.x] = total > 0 ? O / L : 0.f;
-        if (threadIdx.x == 0) { gm[g] = M; gl[g] = L; }
+        if (on && sub == 0) {
+            const float inv = m == -INFINITY ? 0.f : 1.f / l;      // no token at all: zeros
+            reinterpret_cast<float4 *>(a.out + ((size_t)s * a.Hq + h) * kKvD)[lane] =
+                make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        }
+        return;
     }
-    if (!a.weight) return;
+    // weights of the pair (s, j), every w_chunks-th run of slots
+    const int item = blockIdx.x - a.row_ctas, pair = item / a.w_chunks, chunk = item % a.w_chunks;
+    const int s = pair / a.Hkv, j = pair % a.Hkv, n = own_len(a, s);
+    if (chunk * kJoinWarps * kWarp * 4 >= n) return;
+    for (int gq = warp; gq < a.G; gq += kJoinWarps) {
+        const RowPieces x = pieces_of(a, s, j * a.G + gq);
+        const int cnt = x.n_pre + x.n_own;
+        float m = -INFINITY, l = 0.f;
+        for (int i = lane; i < cnt; i += kWarp) {
+            const float *src;
+            const float2 ml = piece_ml(a, x, gq, i, &src);
+            if (src) {
+                const float mx = fmaxf(m, ml.x);
+                l = (m == -INFINITY ? 0.f : l * ex2(m - mx)) + ml.y * ex2(ml.x - mx);
+                m = mx;
+            }
+        }
+        float M = m;
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+        const float L = warp_sum(m == -INFINITY ? 0.f : l * ex2(m - M));
+        if (lane == 0) { gm[gq] = M; gi[gq] = 1.f / L; }
+    }
     __syncthreads();
-    float *w = a.weight + ((size_t)s * a.Hkv + j) * a.max_ctx;
-    for (int t = warp; t < n; t += 4) {
-        float p = 0.f;
-        for (int g = 0; g < a.G; ++g) {
-            const float4 q = *reinterpret_cast<const float4 *>(a.q + s * a.q_stride + (size_t)(j * a.G + g) * kKvD +
-                                                               4 * lane);
-            p += expf(score(q, a.n_prefix + t) - gm[g]) / gl[g];
+    float *wt = a.weight + (size_t)pair * a.max_ctx;
+    const float *sc = a.score + ((size_t)s * a.Hq + (size_t)j * a.G) * a.max_ctx;
+    const int run = kJoinWarps * kWarp * 4;
+    for (int t0 = chunk * run; t0 < n; t0 += a.w_chunks * run) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int t = t0 + k * kJoinWarps * kWarp + tid;
+            if (t < n) {
+                float w = a.decay == 0.f ? 0.f : a.decay * wt[t];
+                for (int gq = 0; gq < a.G; ++gq)
+                    w = fmaf(ex2(__ldcg(sc + (size_t)gq * a.max_ctx + t) - gm[gq]), gi[gq], w);
+                wt[t] = w;
+            }
         }
-        if (lane == 0) w[t] = a.decay == 0.f ? p : a.decay * w[t] + p;
     }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encoder() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(p);
+    });
+    return fn;
+}
+
+// The prefix [n][Hkv][128] f16 as (dim, kv head, token) with a box of 128
+// tokens by 64 dims, 128-byte swizzle; tokens past n come in as zeros.
+int encode_prefix(CUtensorMap *m, const void *base, int Hkv, int n) {
+    EncodeTiledFn fn = encoder();
+    if (!fn) return LI_ERR_UNSUPPORTED;
+    const cuuint64_t dims[3] = {(cuuint64_t)kKvD, (cuuint64_t)Hkv, (cuuint64_t)n};
+    const cuuint64_t strides[2] = {(cuuint64_t)kKvD * 2, (cuuint64_t)Hkv * kKvD * 2};
+    const cuuint32_t box[3] = {64, 1, (cuuint32_t)kPreTok};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : LI_ERR_BAD_SHAPE;
+}
+
+size_t al256(size_t v) { return (v + 255) / 256 * 256; }
+
+// Grids and the workspace of a call; everything the size needs, nothing on
+// the device. Returns the workspace's bytes, 0 when a count is beyond the
+// kernels' integers.
+size_t plan(const li_kv_cache *C, int n_q_heads, KvAttnArgs *a, size_t *off /* [6] */) {
+    const int sms = num_sms();
+    a->B = C->n_seqs; a->Hq = n_q_heads; a->Hkv = C->n_kv_heads; a->G = n_q_heads / C->n_kv_heads;
+    a->max_ctx = C->max_ctx; a->n_prefix = C->n_prefix;
+    const int64_t pairs = (int64_t)a->B * a->Hkv, most = pairs * ((a->max_ctx + kOwnTok - 1ll) / kOwnTok);
+    if (most >= (1ll << 30) || pairs * a->G >= (1ll << 30)) return 0;
+    int64_t grid = most / kOwnMinSteps;
+    grid = grid < 1 ? 1 : grid < sms ? grid : sms;
+    a->own_warps = (int)grid * kOwnWarps;
+    size_t at = 0;
+    off[0] = at; at += al256(((size_t)a->B + 1) * 4);
+    const size_t own_recs = (size_t)pairs + a->own_warps;
+    off[1] = at; at += al256(own_recs * a->G * sizeof(float2));
+    off[2] = at; at += al256(own_recs * a->G * kKvD * 4);
+    off[3] = at; at += C->weight ? al256((size_t)a->B * a->Hq * a->max_ctx * 4) : 0;
+    off[4] = off[5] = at;
+    if (a->n_prefix > 0) {
+        a->rows = a->B * a->G;
+        a->n_rt = (a->rows + kPreRows - 1) / kPreRows;
+        a->n_tt = (a->n_prefix + kPreTok - 1) / kPreTok;
+        const int64_t cost = (int64_t)a->Hkv * a->n_rt * a->n_tt;
+        if (cost >= (1ll << 30)) return 0;
+        // two row tiles share the K and V tiles they read, unless that leaves SMs idle
+        a->per_group = a->n_rt > 1 && cost >= 2ll * sms ? 2 : 1;
+        a->n_grp = (a->n_rt + a->per_group - 1) / a->per_group;
+        a->slots = a->per_group == 2 ? kPreSlots2 : kPreSlots1;
+        a->pre_ctas = (int)(cost < sms ? cost : sms);
+        const size_t recs = ((size_t)a->Hkv * a->n_grp + a->pre_ctas) * 2 * kPreRows;
+        off[4] = at; at += al256(recs * sizeof(float2));
+        off[5] = at; at += al256(recs * kKvD * 4);
+    }
+    return at;
+}
+
+template <int NG, bool SCORE>
+int launch_own(const KvAttnArgs &a, cudaStream_t s) {
+    const cudaError_t e = cudaFuncSetAttribute(kv_own_kernel<NG, SCORE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)kOwnSmem);
+    if (e != cudaSuccess) return (int)e;
+    return (int)launch_pdl(kv_own_kernel<NG, SCORE>, dim3((unsigned)(a.own_warps / kOwnWarps)), dim3(kOwnThreads),
+                           kOwnSmem, s, true, a);
 }
 
 }  // namespace
@@ -94,8 +1148,12 @@ using namespace li;
 extern "C" {
 
 size_t li_attn_kv_workspace_size(const li_kv_cache *C, int n_q_heads) {
-    if (check_kv_cache(C) || C->n_seqs == 0 || n_q_heads <= 0) return 0;
-    return 256;
+    if (check_kv_cache(C) || C->n_seqs == 0 || n_q_heads <= 0 || n_q_heads % C->n_kv_heads ||
+        n_q_heads / C->n_kv_heads > 16)
+        return 0;
+    KvAttnArgs a = {};
+    size_t off[6];
+    return plan(C, n_q_heads, &a, off);
 }
 
 int li_launch_attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_stride, int n_q_heads, float scale,
@@ -106,17 +1164,62 @@ int li_launch_attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_str
     if (n_q_heads / C->n_kv_heads > 16) return LI_ERR_UNSUPPORTED;
     if (!aligned16(q) || !aligned16(out) || q_stride % 4) return LI_ERR_MISALIGNED;
     if (C->n_seqs == 0) return 0;
-    if (!workspace || workspace_bytes < li_attn_kv_workspace_size(C, n_q_heads)) return LI_ERR_WORKSPACE;
-    if (!aligned16(workspace)) return LI_ERR_MISALIGNED;
     KvAttnArgs a = {};
+    size_t off[6];
+    const size_t need = plan(C, n_q_heads, &a, off);
+    if (need == 0) return LI_ERR_BAD_SHAPE;
+    if (!workspace || workspace_bytes < need) return LI_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return LI_ERR_MISALIGNED;
+    const cudaStream_t st = (cudaStream_t)stream;
+    char *ws = static_cast<char *>(workspace);
     a.q = q; a.q_stride = q_stride;
     a.k = static_cast<const __half *>(C->k); a.v = static_cast<const __half *>(C->v);
-    a.kp = static_cast<const __half *>(C->k_prefix); a.vp = static_cast<const __half *>(C->v_prefix);
-    a.len = C->len; a.Hq = n_q_heads; a.Hkv = C->n_kv_heads; a.G = n_q_heads / C->n_kv_heads;
-    a.max_ctx = C->max_ctx; a.n_prefix = C->n_prefix; a.scale = scale; a.decay = decay; a.out = out;
-    a.weight = C->weight;
-    return (int)launch_pdl(kv_attn_kernel, dim3((unsigned)(C->n_seqs * C->n_kv_heads)), dim3(128), 0,
-                           (cudaStream_t)stream, true, a);
+    a.len = C->len;
+    a.cscale = fabsf(scale) * kLog2e; a.qsign = scale < 0.f ? -1.f : 1.f;
+    a.decay = decay; a.out = out; a.weight = C->weight;
+    a.base = reinterpret_cast<int *>(ws + off[0]);
+    a.own_ml = reinterpret_cast<float2 *>(ws + off[1]);
+    a.own_o = reinterpret_cast<float *>(ws + off[2]);
+    a.score = reinterpret_cast<float *>(ws + off[3]);
+    a.pre_ml = reinterpret_cast<float2 *>(ws + off[4]);
+    a.pre_o = reinterpret_cast<float *>(ws + off[5]);
+    a.after_prefix = a.n_prefix > 0;
+    int rc;
+    if (a.n_prefix > 0) {
+        CUtensorMap mk, mv;
+        memset(&mk, 0, sizeof(mk));
+        memset(&mv, 0, sizeof(mv));
+        if ((rc = encode_prefix(&mk, C->k_prefix, a.Hkv, a.n_prefix)) ||
+            (rc = encode_prefix(&mv, C->v_prefix, a.Hkv, a.n_prefix)))
+            return rc;
+        const cudaError_t e = cudaFuncSetAttribute(kv_prefix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)kPreSmem);
+        if (e != cudaSuccess) return (int)e;
+        if ((rc = (int)launch_pdl(kv_prefix_kernel, dim3((unsigned)a.pre_ctas), dim3(kPreThreads), kPreSmem, st, true,
+                                  mk, mv, a)))
+            return rc;
+    }
+    if (a.G <= 8) rc = a.weight ? launch_own<1, true>(a, st) : launch_own<1, false>(a, st);
+    else rc = a.weight ? launch_own<2, true>(a, st) : launch_own<2, false>(a, st);
+    if (rc) return rc;
+    // warps per row: about 16 records each, going by the most a row can have
+    const int pairs = a.B * a.Hkv;
+    const int64_t pre = a.n_prefix ? 2ll * a.pre_ctas / (a.Hkv * a.n_grp) + 2 : 0;
+    int64_t own = (a.max_ctx + kOwnTok - 1) / kOwnTok / kOwnMinSteps + 2;
+    if (own > a.own_warps / pairs + 2) own = a.own_warps / pairs + 2;
+    a.wpr = 1;
+    while (a.wpr < kJoinWarps && a.wpr * 16 < pre + own) a.wpr *= 2;
+    const int per = kJoinWarps / a.wpr;
+    a.row_ctas = (int)(((int64_t)a.B * a.Hq + per - 1) / per);
+    int64_t blocks = a.row_ctas;
+    if (a.weight) {
+        const int run = kJoinWarps * kWarp * 4;
+        int64_t ch = ((int64_t)a.max_ctx + run - 1) / run, cap = ((int64_t)num_sms() * 32 + pairs - 1) / pairs;
+        a.w_chunks = (int)(ch < cap ? ch : cap);
+        blocks += (int64_t)pairs * a.w_chunks;
+    }
+    if (blocks > 0x7fffffff) return LI_ERR_BAD_SHAPE;
+    return (int)launch_pdl(kv_join_kernel, dim3((unsigned)blocks), dim3(kJoinWarps * kWarp), 0, st, true, a);
 }
 
 }  // extern "C"
