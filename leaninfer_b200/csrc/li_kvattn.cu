@@ -62,7 +62,7 @@ constexpr int kScanMax = 2048;                 // entries of the length scan in 
 
 // ---- prefix part -----------------------------------------------------------
 constexpr int kPreRows = 128, kPreTok = 128;
-constexpr int kPreThreads = 384;               // warps 0-3, 4-7: softmax; 8: TMA; 9, 10: MMA of buffer 0, 1
+constexpr int kPreThreads = 384;               // warps 0-3, 4-7: softmax; 8: TMA; 9: MMA
 constexpr int kPreRegsSoft = 208, kPreRegsRest = 88;        // 256 * 208 + 128 * 88 = 384 * 168
 constexpr uint32_t kPreSlotBytes = kPreTok * kKvD * 2;      // 128 tokens of K or V: 32 KB
 constexpr uint32_t kPreQBytes = 2 * kPreRows * kKvD * 2;    // a row tile's hi and lo: 64 KB
@@ -91,10 +91,10 @@ struct KvAttnArgs {
     // prefix part
     int n_prefix, rows, n_rt, per_group, n_grp, n_tt;   // rows = B G; row tiles; row tiles per group; groups; tiles
     int pre_ctas, slots;
-    float2 *pre_ml;                    // [Hkv n_grp + pre_ctas][2][128]
-    float *pre_o;                      // [Hkv n_grp + pre_ctas][2][128][128]
+    float2 *pre_ml;                    // [Hkv n_grp + pre_ctas][2][128 rows]
+    float *pre_o;                      // [Hkv n_grp + pre_ctas][2][32 groups of 4 dims][128 rows][4]
     // join
-    int row_ctas, wpr, w_chunks;       // blocks that join rows, warps per row, blocks per pair that write weights
+    int row_ctas, wpr, w_chunks;       // blocks that join rows, warps per 8 rows, blocks per pair that write weights
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -131,17 +131,27 @@ __device__ __forceinline__ float inv_pow2(float p) {
 }
 
 // ---------------------------------------------------------------------------
-// Pieces of the own part: the steps of all (sequence, kv head) pairs in order
-// (total T) are dealt to W warps in equal runs; warp w has [w T / W, (w+1) T / W).
-// The piece of pair p that warp w holds is record p + w: along the line of
-// steps either p or w grows from piece to piece, so no two share a record.
+// A line of T units dealt to W takers in runs whose lengths differ by at most
+// one: the first T % W takers have T / W + 1.
 // ---------------------------------------------------------------------------
+struct Runs {
+    int len, extra;
+    __device__ __forceinline__ Runs(int T, int W) : len(T / W), extra(T % W) {}
+    __device__ __forceinline__ int begin(int w) const { return w * len + min(w, extra); }
+    __device__ __forceinline__ int taker(int unit) const {          // of a unit on the line
+        const int cut = extra * (len + 1);
+        return unit < cut ? unit / (len + 1) : extra + (unit - cut) / len;
+    }
+};
+
+// Pieces of the own part: the steps of all (sequence, kv head) pairs in order,
+// T of them, are dealt to W warps. The piece of pair p that warp w holds is
+// record p + w: along the line of steps either p or w grows from piece to
+// piece, so no two share a record.
 __device__ __forceinline__ int own_active(int T, int warps) {
     const int w = T / kOwnMinSteps;
     return w < 1 ? 1 : w < warps ? w : warps;
 }
-__device__ __forceinline__ int run_begin(int w, int T, int W) { return (int)((int64_t)w * T / W); }
-__device__ __forceinline__ int run_of(int step, int T, int W) { return (int)((((int64_t)step + 1) * W - 1) / T); }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -228,7 +238,8 @@ __global__ void __launch_bounds__(kOwnThreads, 1) kv_own_kernel(const __grid_con
 
     const int W = own_active(T, a.own_warps);
     const int w = warp * gridDim.x + blockIdx.x;       // neighbouring pieces on different SMs
-    const int lo = w < W && T > 0 ? run_begin(w, T, W) : 0, hi = w < W && T > 0 ? run_begin(w + 1, T, W) : 0;
+    const Runs runs(T, W);
+    const int lo = w < W ? runs.begin(w) : 0, hi = w < W ? runs.begin(w + 1) : 0;
     const int n_steps = hi - lo;
     if (n_steps > 0) {
         // a cursor: sequence, kv head, step within the pair, and the sequence's length
@@ -467,10 +478,10 @@ __device__ __forceinline__ Group group_at(const KvAttnArgs &a, int p) {
     g.base = (g.j * a.n_rt + g.rt) * a.n_tt;
     return g;
 }
-// token tiles [t0, t1) of group g in the run [lo, hi)
-__device__ __forceinline__ void tiles_of(const KvAttnArgs &a, const Group &g, int lo, int hi, int &t0, int &t1) {
-    t0 = lo <= g.base ? 0 : (lo - g.base + g.nt - 1) / g.nt;
-    t1 = hi <= g.base ? 0 : (hi - g.base + g.nt - 1) / g.nt;
+// token tiles [t0, t1) in the run [lo, hi) of a group at `base` with nt (1 or 2) row tiles
+__device__ __forceinline__ void tiles_of(const KvAttnArgs &a, int base, int nt, int lo, int hi, int &t0, int &t1) {
+    t0 = lo <= base ? 0 : (lo - base + nt - 1) >> (nt - 1);
+    t1 = hi <= base ? 0 : (hi - base + nt - 1) >> (nt - 1);
     if (t1 > a.n_tt) t1 = a.n_tt;
 }
 
@@ -503,22 +514,15 @@ __device__ __forceinline__ bool softmax_bar_any(bool v) {
     return r != 0;
 }
 
-// Order in which the K and V tiles of a piece of n token tiles go through the
-// ring: place i = 0 .. 2n-1 holds K or V of token tile t. With two row tiles
-// (nt 2) both buffers use every tile: K0 V0 K1 V1 ...; with one, buffer b takes
-// the tiles t % 2 == b: K0 K1 V0 K2 V1 K3 V2 ...
-__device__ __forceinline__ void ring_place(int i, int n, int nt, int &t, bool &is_v) {
-    if (nt == 2) {
-        t = i >> 1;
-        is_v = i & 1;
-    } else if (i == 2 * n - 1) {
-        t = n - 1;
-        is_v = true;
-    } else {
-        is_v = i > 0 && !(i & 1);
-        t = is_v ? (i - 2) >> 1 : (i + 1) >> 1;
-    }
-}
+// Order in which the products of a piece of n token tiles are issued, and its
+// K and V tiles go through the ring. The units u = 0 .. n nt - 1 are token tile
+// u / 2 of row tile u % 2 (nt 2) or token tile u (nt 1), and unit u runs in
+// score buffer u % 2: scores of units 0 and 1, then for each u P V of u and the
+// scores of u + 2, which take the buffer that P of u leaves. So each buffer's
+// softmax runs under the other's products. Tiles, by first use:
+//   nt 2: K0 V0 K1 V1 ...;   nt 1: K0 K1 V0 K2 V1 K3 V2 ...
+__device__ __forceinline__ int k_place(int t, int nt) { return nt == 2 ? 2 * t : t == 0 ? 0 : 2 * t - 1; }
+__device__ __forceinline__ int v_place(int t, int nt, int n) { return nt == 2 ? 2 * t + 1 : t + (t + 2 < n ? t + 2 : n); }
 
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
@@ -538,16 +542,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// Adds to global memory without waiting. A record's words are only ever
-// touched by one thread, so its sums have one order.
-__device__ __forceinline__ void red_add4(float4 *p, float a, float b, float c, float d) {
-    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(a), "f"(b), "f"(c), "f"(d)
-                 : "memory");
-}
-__device__ __forceinline__ void red_add2(float2 *p, float a, float b) {
-    asm volatile("red.relaxed.gpu.global.add.v2.f32 [%0], {%1, %2};" ::"l"(p), "f"(a), "f"(b) : "memory");
-}
-
 __global__ void __launch_bounds__(kPreThreads, 1)
 kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const __grid_constant__ KvAttnArgs a) {
@@ -557,20 +551,21 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     uint8_t *ring = smem + (size_t)a.per_group * kPreQBytes;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + 2 * kPreQBytes + kPreSlots2 * kPreSlotBytes);
     uint64_t *full = bars, *empty = full + kPreSlots1, *q_full = empty + kPreSlots1, *s_full = q_full + 1,
-             *p_full = s_full + 2, *o_full = p_full + 2, *fin = o_full + 2;
+             *p_full = s_full + 2, *o_full = p_full + 4, *turn = o_full + 2, *fin = turn + 2;
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(fin + 2);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
     const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
     const int slots = a.slots;
     if (tid == 0) {
-        for (int i = 0; i < slots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 2); }
+        for (int i = 0; i < slots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], a.per_group); }
         mbar_init(q_full, 8);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
             mbar_init(&o_full[i], 1);
+            mbar_init(&turn[i], 1);
             mbar_init(&fin[i], 1);
         }
+        for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 4);      // [buffer][64 tokens]
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -583,7 +578,8 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     grid_dep_launch_dependents();
 
     const int cost = a.Hkv * a.n_rt * a.n_tt, c = blockIdx.x;
-    const int lo = (int)((int64_t)cost * c / a.pre_ctas), hi = (int)((int64_t)cost * (c + 1) / a.pre_ctas);
+    const Runs runs(cost, a.pre_ctas);
+    const int lo = runs.begin(c), hi = runs.begin(c + 1);
     int p0;                                                        // the group that lo falls into
     {
         const int per_j = a.n_rt * a.n_tt, j = lo / per_j;
@@ -604,21 +600,22 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 const Group g = group_at(a, p);
                 if (g.base >= hi) break;
                 int t0, t1;
-                tiles_of(a, g, lo, hi, t0, t1);
+                tiles_of(a, g.base, g.nt, lo, hi, t0, t1);
                 const int n = t1 - t0;
-                for (int i = 0; i < 2 * n; ++i) {
-                    int t;
-                    bool is_v;
-                    ring_place(i, n, g.nt, t, is_v);
-                    if (used >= slots && !(ok = wait_or_abort(&empty[slot], par, abort_flag))) break;
+                auto load = [&](const CUtensorMap *map, int t) {
+                    if (used >= slots && !(ok = ok && wait_or_abort(&empty[slot], par, abort_flag))) return;
                     mbar_arrive_expect_tx(&full[slot], kPreSlotBytes);
                     uint8_t *dst = ring + (size_t)slot * kPreSlotBytes;
-                    const CUtensorMap *map = is_v ? &tmV : &tmK;
                     const int z = (t0 + t) * kPreTok;
                     tma_load_3d(dst, map, 0, g.j, z, &full[slot]);
                     tma_load_3d(dst + kPreSlotBytes / 2, map, 64, g.j, z, &full[slot]);
                     ++used;
                     if (++slot == slots) { slot = 0; par ^= 1u; }
+                };
+                for (int t = 0; ok && t < n; ++t) {
+                    if (g.nt == 2 || t == 0) load(&tmK, t);
+                    if (g.nt == 1 && t + 1 < n) load(&tmK, t + 1);
+                    load(&tmV, t);
                 }
             }
             // every copy issued has landed before the block ends
@@ -627,69 +624,105 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         } else if ((warp == 9 || warp == 10) && lane == 0) {
             // ---------------- MMA issuer of buffer b ----------------
             // The thread stands still while an MMA is taken, so what it does
-            // between them adds to the tensor pipe's time; the two issuers
-            // cover for each other, and descriptors advance by constants.
+            // between them adds to the tensor pipe's time: descriptors advance
+            // by constants, and the two issuers take turns, a batch (P V of a
+            // unit, scores of the next) each, one's waits and commits running
+            // under the other's products. Without turns the two batches would
+            // mix, end together, and leave the tensor pipe idle while both
+            // buffers' softmax runs.
             const int b = warp - 9;
             const uint32_t id_s = idesc_kf16(128, kPreTok, false);
             const uint32_t id_o = idesc_kf16(128, kKvD, false) | kIdescBMajorMN;
             const uint64_t k0 = sw128_desc(smem_addr(ring)), v0 = sw128_mn_desc(smem_addr(ring), kPreSlotBytes / 2);
             const uint32_t ts = tmem + 128u * b, to = tmem + 256u + 128u * b;
-            int slot = 0;
-            uint32_t par = 0, pq = 0, pp = 0;                      // phases of the slot, q_full, p_full
-            bool ok = true;
+            struct Place { int slot; uint32_t par; };              // a ring place's slot and the phase of its copy
+            auto advance = [&](Place &x, int by) {
+                x.slot += by;
+                while (x.slot >= slots) { x.slot -= slots; x.par ^= 1u; }
+            };
+            int place0 = 0;                                        // ring places before this piece
+            uint32_t pq = 0, pp = 0, pt = 0;                       // phases of q_full, p_full, turn
+            bool ok = true, have = b == 0;
+            auto acquire = [&]() -> bool {
+                if (!have && !wait_or_abort(&turn[b], pt, abort_flag)) return false;
+                if (!have) pt ^= 1u;
+                return have = true;
+            };
+            auto pass = [&]() {
+                mbar_arrive(&turn[b ^ 1]);
+                have = false;
+            };
             for (int p = p0; ok && p < p_end; ++p) {
                 const Group g = group_at(a, p);
                 if (g.base >= hi) break;
                 int t0, t1;
-                tiles_of(a, g, lo, hi, t0, t1);
-                const int n = t1 - t0;
+                tiles_of(a, g.base, g.nt, lo, hi, t0, t1);
+                const int n = t1 - t0, U = n * g.nt;
                 if (n <= 0) continue;
                 if (!(ok = wait_or_abort(q_full, pq, abort_flag))) break;
                 pq ^= 1u;
-                const uint64_t q_hi = sw128_desc(smem_addr(qbuf) + (g.nt == 2 ? (uint32_t)b * kPreQBytes : 0u));
-                const int last = g.nt == 2 || ((n - 1) & 1) == b ? n - 1 : n - 2;      // this buffer's last tile
-                int unit = 0;
-                for (int i = 0; i < 2 * n; ++i) {
-                    int t;
-                    bool is_v;
-                    ring_place(i, n, g.nt, t, is_v);
-                    const bool mine = g.nt == 2 || (t & 1) == b;
-                    if (mine && is_v) {
-                        if (!(ok = wait_or_abort(&p_full[b], pp, abort_flag))) break;
-                        pp ^= 1u;
-                    }
-                    if (!(ok = wait_or_abort(&full[slot], par, abort_flag))) break;
-                    if (!mine) {
-                        mbar_arrive(&empty[slot]);
-                    } else if (!is_v) {
-                        // S = Q K^T; lo first, so that only the hi products add to a sum of full size (the
-                        // tensor cores' sums round towards zero, once per instruction)
-                        tc_fence_after();
-                        const uint64_t kd = k0 + (uint64_t)(slot * (kPreSlotBytes >> 4));
-#pragma unroll
-                        for (int x = 0; x < 16; ++x) {
-                            const uint32_t at = 1024u * ((x & 7) >> 2) + 2u * (x & 3);
-                            umma_f16(ts, q_hi + (x < 8 ? 2048u : 0u) + at, kd + at, id_s, x ? 1u : 0u);
-                        }
-                        umma_commit(&s_full[b]);
-                        umma_commit(&empty[slot]);
-                    } else {
-                        tc_fence_after();
-                        const uint64_t vd = v0 + (uint64_t)(slot * (kPreSlotBytes >> 4));
-                        const uint32_t again = unit % kPreFlush ? 1u : 0u;
-#pragma unroll
-                        for (int x = 0; x < 16; ++x)
-                            umma_f16_ta(to, ts + (x < 8 ? 64u : 0u) + 8u * (x & 7), vd + 128u * (x & 7), id_o,
-                                        x ? 1u : again);
-                        if (t == last) umma_commit(&o_full[b]);
-                        umma_commit(&empty[slot]);
-                        ++unit;
-                    }
-                    if (++slot == slots) { slot = 0; par ^= 1u; }
+                const uint64_t qd = sw128_desc(smem_addr(qbuf) + (g.nt == 2 ? (uint32_t)b * kPreQBytes : 0u));
+                auto place = [&](int at) { return Place{at % slots, (uint32_t)((at / slots) & 1)}; };
+                const int tb = g.nt == 2 ? 0 : b;                  // this buffer's first tile
+                Place kp = place(place0 + k_place(tb, g.nt)), vp = place(place0 + v_place(tb, g.nt, n));
+                place0 += 2 * n;
+                if (b >= U) {                                      // one unit: nothing for buffer 1, but o_full counts
+                    mbar_arrive(&o_full[b]);                       // pieces, so that no issuer falls a piece behind
+                    continue;
                 }
-                // a piece of one tile leaves buffer 1 nothing to do; o_full counts pieces all the same, so that no
-                // issuer falls a piece behind
-                if (last < 0) mbar_arrive(&o_full[b]);
+                auto release = [&](int slot) {
+                    umma_commit(&empty[slot]);
+                    if (g.nt < a.per_group) umma_commit(&empty[slot]);     // for the buffer that does not use it
+                };
+                // scores of unit u; lo first, so that only the hi products add to a sum of full size (the tensor
+                // cores' sums round towards zero, once per instruction)
+                auto scores = [&](uint64_t kd) {
+                    tc_fence_after();
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const uint32_t k = 1024u * ((x & 7) >> 2) + 2u * (x & 3);
+                        umma_f16(ts, qd + (x < 8 ? 2048u : 0u) + k, kd + k, id_s, x ? 1u : 0u);
+                    }
+                };
+                if (!(ok = wait_or_abort(&full[kp.slot], kp.par, abort_flag) && acquire())) break;
+                scores(k0 + (uint64_t)(kp.slot * (kPreSlotBytes >> 4)));
+                if (b == 1 || U > 1) pass();
+                umma_commit(&s_full[b]);
+                release(kp.slot);
+                for (int u = b; u < U; u += 2) {
+                    const int t = g.nt == 2 ? u >> 1 : u;
+                    const uint64_t vd = v0 + (uint64_t)(vp.slot * (kPreSlotBytes >> 4));
+                    const uint32_t again = (u >> 1) % kPreFlush ? 1u : 0u;
+                    const bool more = u + 2 < U;
+                    if (!(ok = wait_or_abort(&full[vp.slot], vp.par, abort_flag) &&
+                               wait_or_abort(&p_full[2 * b], pp, abort_flag) && acquire()))
+                        break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        umma_f16_ta(to, ts + (x < 4 ? 64u : 0u) + 8u * (x & 3), vd + 128u * (x & 3), id_o, x ? 1u : again);
+                    // the first 64 tokens' products run while the softmax ends the other half
+                    if (more) {
+                        advance(kp, g.nt == 2 ? 2 : k_place(t + 2, 1) - k_place(t, 1));
+                        ok = wait_or_abort(&full[kp.slot], kp.par, abort_flag);
+                    }
+                    if (!(ok = ok && wait_or_abort(&p_full[2 * b + 1], pp, abort_flag))) break;
+                    pp ^= 1u;
+                    tc_fence_after();
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        umma_f16_ta(to, ts + (x < 4 ? 64u : 0u) + 32u + 8u * (x & 3), vd + 512u + 128u * (x & 3), id_o, 1u);
+                    // o goes to the record: the buffer's last unit, or kPreFlush of them summed
+                    if (!more || (u >> 1) % kPreFlush == kPreFlush - 1) umma_commit(&o_full[b]);
+                    if (more) scores(k0 + (uint64_t)(kp.slot * (kPreSlotBytes >> 4)));
+                    if (u + 1 < U || b == 1) pass();               // an odd piece ends with buffer 0, which begins the next
+                    if (more) umma_commit(&s_full[b]);
+                    release(vp.slot);
+                    if (more) {
+                        release(kp.slot);
+                        advance(vp, g.nt == 2 ? 2 : v_place(t + 2, 1, n) - v_place(t, 1, n));
+                    }
+                }
             }
             umma_commit(&fin[b]);
             mbar_wait(&fin[b], 0u);
@@ -706,7 +739,7 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             const Group g = group_at(a, p);
             if (g.base >= hi) break;
             int t0, t1;
-            tiles_of(a, g, lo, hi, t0, t1);
+            tiles_of(a, g.base, g.nt, lo, hi, t0, t1);
             const int n = t1 - t0;
             if (n <= 0) continue;
             // this row's q: scaled, split and stored as the operand's rows
@@ -750,34 +783,38 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             if (lane == 0) mbar_arrive(q_full);
             float m = -INFINITY, l = 0.f, m_rec = -INFINITY;
             bool ok = true;
-            const size_t rec = ((size_t)(p + c) * 2 + b) * kPreRows + r;
-            float4 *d = reinterpret_cast<float4 *>(a.pre_o + rec * kKvD);
-            // o in tensor memory joins this row of the record, whose values have the factor 2^(m_rec)
-            auto flush = [&]() {
-                const float fr = m_rec == -INFINITY ? 0.f : ex2(m_rec - m);
+            const size_t rec = ((size_t)(p + c) * 2 + b) * kPreRows;
+            float4 *d = reinterpret_cast<float4 *>(a.pre_o + rec * kKvD) + r;      // [32 groups of 4 dims][128 rows]
+            // o in tensor memory joins this row of the record, whose values have the factor 2^(m_rec); the record's
+            // old values are fetched while the products run
+            auto flush = [&]() -> bool {
+                float4 old[32];
+                const bool again = m_rec != -INFINITY;
+                const float fr = again ? ex2(m_rec - m) : 0.f;
+#pragma unroll
+                for (int x = 0; x < 32; ++x) old[x] = again && live ? __ldcg(d + x * kPreRows) : make_float4(0.f, 0.f, 0.f, 0.f);
+                if (!__all_sync(0xffffffffu, wait_or_abort(&o_full[b], po, abort_flag))) return false;
+                po ^= 1u;
+                tc_fence_after();
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     uint32_t ov[32];
                     tmem_ld32_nowait(ob + 32u * x, ov);
                     tmem_wait_ld();
-                    if (!live) continue;
+                    if (live)
 #pragma unroll
-                    for (int y = 0; y < 8; ++y) {
-                        float4 w = make_float4(__uint_as_float(ov[4 * y]), __uint_as_float(ov[4 * y + 1]),
-                                               __uint_as_float(ov[4 * y + 2]), __uint_as_float(ov[4 * y + 3]));
-                        if (m_rec == m) {
-                            red_add4(d + 8 * x + y, w.x, w.y, w.z, w.w);
-                            continue;
+                        for (int y = 0; y < 8; ++y) {
+                            const float4 w = old[8 * x + y];
+                            __stcg(d + (8 * x + y) * kPreRows,
+                                   make_float4(fmaf(w.x, fr, __uint_as_float(ov[4 * y])),
+                                               fmaf(w.y, fr, __uint_as_float(ov[4 * y + 1])),
+                                               fmaf(w.z, fr, __uint_as_float(ov[4 * y + 2])),
+                                               fmaf(w.w, fr, __uint_as_float(ov[4 * y + 3]))));
                         }
-                        if (m_rec != -INFINITY) {
-                            const float4 old = __ldcg(d + 8 * x + y);
-                            w.x = fmaf(old.x, fr, w.x); w.y = fmaf(old.y, fr, w.y);
-                            w.z = fmaf(old.z, fr, w.z); w.w = fmaf(old.w, fr, w.w);
-                        }
-                        __stcg(d + 8 * x + y, w);
-                    }
                 }
+                tc_fence_before();
                 m_rec = m;
+                return true;
             };
             int unit = 0;
             // this buffer's token tiles: every one (nt 2), or every second one
@@ -787,8 +824,6 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 if (!ok) break;
                 ps ^= 1u;
                 tc_fence_after();
-                // P V of this buffer's last tile is complete: these scores were issued after it
-                if (unit > 0 && unit % kPreFlush == 0) flush();
                 uint32_t v[4][32];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) tmem_ld32_nowait(sb + 32u * x, v[x]);
@@ -820,6 +855,7 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 if (grow) m = mx;
                 l *= f;
                 if (unit % kPreFlush && __any_sync(0xffffffffu, grow)) {
+                    // P V of this buffer's last tile is complete: these scores were issued after it
                     for (int x = 0; x < 4; ++x) {
                         uint32_t ov[32];
                         tmem_ld32_nowait(ob + 32u * x, ov);
@@ -851,27 +887,27 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                     }
                     tmem_st32(sb + 32u * hf, hw);
                     tmem_st32(sb + 64u + 32u * hf, lw);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * b + hf]);
                 }
                 {
                     float l0, l1;
                     unpack2(add2(add2(ls[0], ls[1]), add2(ls[2], ls[3])), l0, l1);
                     l += l0 + l1;
                 }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[b]);
-            }
-            if (ok) {
-                ok = __all_sync(0xffffffffu, wait_or_abort(&o_full[b], po, abort_flag));
-                po ^= 1u;
-                if (ok && first < n) {
-                    tc_fence_after();
-                    flush();
-                    if (live) a.pre_ml[rec] = make_float2(m - kPShift, l);
-                    tc_fence_before();
+                // P V of this unit ends a sum: the buffer's last, or kPreFlush of them
+                if (i + step >= n || unit % kPreFlush == kPreFlush - 1) {
+                    ok = flush();
+                    if (!ok) break;
                 }
             }
+            if (ok && first >= n) {
+                ok = __all_sync(0xffffffffu, wait_or_abort(&o_full[b], po, abort_flag));
+                po ^= 1u;
+            }
+            if (ok && live && first < n) a.pre_ml[rec + r] = make_float2(m - kPShift, l);
             // both buffers are done with q before the next piece's is written
             stop = softmax_bar_any(!ok);
         }
@@ -887,132 +923,140 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 }
 
 // ---------------------------------------------------------------------------
-// The join. Record i of row (s, h): the prefix's pieces first, then the own
-// part's; returns its place, or -1 for a piece that holds no token.
+// The join of the pieces of row r = s G + g of kv head j. Pieces 0 .. n_pre-1
+// are the prefix's (the same for all rows of a row tile), then the own part's.
 // ---------------------------------------------------------------------------
 struct RowPieces {
     int n_pre, n_own;
-    // prefix
-    Group g;
-    int p, c0, streams, stream0, prow;
-    // own
-    int rec0;
+    int p, c0, streams, stream0, prow;     // prefix: group, first block, records per block
+    int len, extra, base, nt;              //         the blocks' runs, the group's place and cost
+    int rec0, gq;                          // own
 };
 
-__device__ __forceinline__ RowPieces pieces_of(const KvAttnArgs &a, int s, int h) {
+__device__ __forceinline__ RowPieces pieces_of(const KvAttnArgs &a, int j, int row) {
     RowPieces x;
-    const int j = h / a.G, gq = h - j * a.G;
+    const int s = row / a.G;
+    x.gq = row - s * a.G;
     x.n_pre = x.n_own = 0;
+    const int n = own_len(a, s), T = __ldcg(a.base + a.B), b0 = __ldcg(a.base + s);
     if (a.n_prefix > 0) {
-        const int row = s * a.G + gq, rt = row / kPreRows;
+        const int rt = row / kPreRows;
         x.prow = row - rt * kPreRows;
         x.p = j * a.n_grp + rt / a.per_group;
-        x.g = group_at(a, x.p);
-        const int cost = a.Hkv * a.n_rt * a.n_tt;
-        x.c0 = run_of(x.g.base, cost, a.pre_ctas);
-        const int c1 = run_of(x.g.base + x.g.nt * a.n_tt - 1, cost, a.pre_ctas);
-        x.streams = x.g.nt == 2 ? 1 : 2;
-        x.stream0 = x.g.nt == 2 ? rt - x.g.rt : 0;
+        const Group g = group_at(a, x.p);
+        const Runs runs(a.Hkv * a.n_rt * a.n_tt, a.pre_ctas);
+        x.len = runs.len; x.extra = runs.extra; x.base = g.base; x.nt = g.nt;
+        x.c0 = runs.taker(g.base);
+        const int c1 = runs.taker(g.base + g.nt * a.n_tt - 1);
+        x.streams = g.nt == 2 ? 1 : 2;
+        x.stream0 = g.nt == 2 ? rt - g.rt : 0;
         x.n_pre = (c1 - x.c0 + 1) * x.streams;
     }
-    const int n = own_len(a, s);
     if (n > 0) {
-        const int T = __ldcg(a.base + a.B), W = own_active(T, a.own_warps), st = own_steps(n);
-        const int b0 = __ldcg(a.base + s) + j * st;
-        const int w0 = run_of(b0, T, W), w1 = run_of(b0 + st - 1, T, W);
+        const Runs runs(T, own_active(T, a.own_warps));
+        const int st = own_steps(n), at = b0 + j * st;
+        const int w0 = runs.taker(at), w1 = runs.taker(at + st - 1);
         x.rec0 = s * a.Hkv + j + w0;
         x.n_own = w1 - w0 + 1;
     }
     return x;
 }
 
-// (max, sum) of record i; its o in *o. (-inf, 0) for an empty one.
-__device__ __forceinline__ float2 piece_ml(const KvAttnArgs &a, const RowPieces &x, int gq, int i, const float **o) {
-    if (i < x.n_pre) {
-        const int c = x.c0 + i / x.streams, w = x.stream0 + i % x.streams;
-        const int cost = a.Hkv * a.n_rt * a.n_tt;
-        int t0, t1;
-        tiles_of(a, x.g, (int)((int64_t)cost * c / a.pre_ctas), (int)((int64_t)cost * (c + 1) / a.pre_ctas), t0, t1);
-        if (t1 - t0 <= (x.streams == 2 ? w : 0)) {
-            *o = nullptr;
-            return make_float2(-INFINITY, 0.f);
-        }
-        const size_t rec = ((size_t)(x.p + c) * 2 + w) * kPreRows + x.prow;
-        *o = a.pre_o + rec * kKvD;
-        return __ldcg(a.pre_ml + rec);
-    }
-    const size_t rec = (size_t)(x.rec0 + i - x.n_pre) * a.G + gq;
-    *o = a.own_o + rec * kKvD;
-    return __ldcg(a.own_ml + rec);
+// Record of prefix piece i, or -1 where that piece holds no token.
+__device__ __forceinline__ int pre_record(const KvAttnArgs &a, const RowPieces &x, int i) {
+    const int c = x.c0 + (x.streams == 2 ? i >> 1 : i), w = x.streams == 2 ? i & 1 : x.stream0;
+    const int lo = c * x.len + min(c, x.extra), hi = (c + 1) * x.len + min(c + 1, x.extra);
+    int t0, t1;
+    tiles_of(a, x.base, x.nt, lo, hi, t0, t1);
+    return t1 - t0 > (x.streams == 2 ? w : 0) ? (x.p + c) * 2 + w : -1;
 }
 
-constexpr int kJoinWarps = 8;
+// (max, sum) of piece i; (-inf, 0) for an empty one.
+__device__ __forceinline__ float2 piece_ml(const KvAttnArgs &a, const RowPieces &x, int i) {
+    if (i < x.n_pre) {
+        const int rec = pre_record(a, x, i);
+        return rec < 0 ? make_float2(-INFINITY, 0.f) : __ldcg(a.pre_ml + (size_t)rec * kPreRows + x.prow);
+    }
+    return __ldcg(a.own_ml + (size_t)(x.rec0 + i - x.n_pre) * a.G + x.gq);
+}
 
+constexpr int kJoinWarps = 8, kJoinRows = 8;
+
+// Rows: wpr neighbouring warps take 8 rows of a kv head, each its share of the
+// pieces; lane l holds row l % 8 and dims 16 i + 4 (l / 8) .. +3, i < 8, so that
+// a load reads 128 contiguous bytes of each of four dim groups.
 __global__ void __launch_bounds__(kJoinWarps * kWarp) kv_join_kernel(const __grid_constant__ KvAttnArgs a) {
-    __shared__ float red_m[kJoinWarps], red_l[kJoinWarps];
-    __shared__ __align__(16) float red_o[kJoinWarps][kKvD];
+    __shared__ float red_m[kJoinWarps][kJoinRows], red_l[kJoinWarps][kJoinRows];
+    __shared__ __align__(16) float4 red_o[kJoinWarps][8][kWarp];
     __shared__ float gm[16], gi[16];
     grid_dep_wait();
     grid_dep_launch_dependents();
     const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
     if ((int)blockIdx.x < a.row_ctas) {
-        // a row (s, h) on wpr neighbouring warps, each over its share of the records
         const int per = kJoinWarps / a.wpr, sub = warp % a.wpr;
-        const int64_t rowi = (int64_t)blockIdx.x * per + warp / a.wpr;
-        const bool on = rowi < (int64_t)a.B * a.Hq;
+        const int rows = a.B * a.G, blocks = (rows + kJoinRows - 1) / kJoinRows;      // row blocks of a kv head
+        const int item = blockIdx.x * per + warp / a.wpr, j = item / blocks;
+        const int rl = lane & 7, xq = lane >> 3, row = (item - j * blocks) * kJoinRows + rl;
+        const bool on = j < a.Hkv && row < rows;
         float m = -INFINITY, l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        const int s = on ? (int)(rowi / a.Hq) : 0, h = on ? (int)(rowi - (int64_t)s * a.Hq) : 0;
-        if (on) {
-            const RowPieces x = pieces_of(a, s, h);
-            const int n = x.n_pre + x.n_own, gq = h % a.G;
-            for (int i0 = sub * kWarp; i0 < n; i0 += a.wpr * kWarp) {
-                const float *src = nullptr;
-                const float2 ml = i0 + lane < n ? piece_ml(a, x, gq, i0 + lane, &src) : make_float2(-INFINITY, 0.f);
-                float mx = ml.x;
+        float4 o[8];
 #pragma unroll
-                for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-                mx = fmaxf(mx, m);
-                const float keep = m == -INFINITY ? 0.f : ex2(m - mx), f = src ? ex2(ml.x - mx) : 0.f;
-                m = mx;
-                l = l * keep + warp_sum(f * ml.y);
-                o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
-                const int cnt = min(kWarp, n - i0);
-#pragma unroll 4
-                for (int k = 0; k < cnt; ++k) {
-                    const float fk = __shfl_sync(0xffffffffu, f, k);
-                    const float *ok = reinterpret_cast<const float *>(
-                        __shfl_sync(0xffffffffu, (unsigned long long)reinterpret_cast<uintptr_t>(src), k));
-                    if (ok) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(ok) + lane);
-                        o.x = fmaf(fk, v.x, o.x); o.y = fmaf(fk, v.y, o.y);
-                        o.z = fmaf(fk, v.z, o.z); o.w = fmaf(fk, v.w, o.w);
-                    }
+        for (int i = 0; i < 8; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (on) {
+            const RowPieces x = pieces_of(a, j, row);
+            const int n = x.n_pre + x.n_own;
+            for (int i = sub; i < n; i += a.wpr) m = fmaxf(m, piece_ml(a, x, i).x);
+#pragma unroll 2
+            for (int i = sub; i < n; i += a.wpr) {
+                const float2 ml = piece_ml(a, x, i);
+                const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+                l = fmaf(f, ml.y, l);
+                const float4 *src = nullptr;
+                int step = 0;
+                if (i >= x.n_pre) {
+                    src = reinterpret_cast<const float4 *>(a.own_o + ((size_t)(x.rec0 + i - x.n_pre) * a.G + x.gq) * kKvD) + xq;
+                    step = 4;
+                } else if (const int rec = pre_record(a, x, i); rec >= 0) {
+                    src = reinterpret_cast<const float4 *>(a.pre_o) + ((size_t)rec * 32 + xq) * kPreRows + x.prow;
+                    step = 4 * kPreRows;
                 }
+                if (src)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float4 v = __ldcg(src + k * step);
+                        o[k].x = fmaf(f, v.x, o[k].x); o[k].y = fmaf(f, v.y, o[k].y);
+                        o[k].z = fmaf(f, v.z, o[k].z); o[k].w = fmaf(f, v.w, o[k].w);
+                    }
             }
         }
         if (a.wpr > 1) {
-            if (lane == 0) { red_m[warp] = m; red_l[warp] = l; }
-            reinterpret_cast<float4 *>(red_o[warp])[lane] = o;
+            if (xq == 0) { red_m[warp][rl] = m; red_l[warp][rl] = l; }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) red_o[warp][k][lane] = o[k];
             __syncthreads();
             if (sub == 0) {
                 float M = m;
-                for (int k = 1; k < a.wpr; ++k) M = fmaxf(M, red_m[warp + k]);
-                const float f0 = m == -INFINITY ? 0.f : ex2(m - M);
-                l *= f0;
-                o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
-                for (int k = 1; k < a.wpr; ++k) {
-                    const float f = red_m[warp + k] == -INFINITY ? 0.f : ex2(red_m[warp + k] - M);
-                    const float4 v = reinterpret_cast<const float4 *>(red_o[warp + k])[lane];
-                    l = fmaf(f, red_l[warp + k], l);
-                    o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+                for (int w = 1; w < a.wpr; ++w) M = fmaxf(M, red_m[warp + w][rl]);
+                for (int w = 0; w < a.wpr; ++w) {
+                    const float f = red_m[warp + w][rl] == -INFINITY ? 0.f : ex2(red_m[warp + w][rl] - M);
+                    l = w ? fmaf(f, red_l[warp + w][rl], l) : f * l;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float4 v = red_o[warp + w][k][lane];
+                        o[k].x = w ? fmaf(f, v.x, o[k].x) : f * v.x; o[k].y = w ? fmaf(f, v.y, o[k].y) : f * v.y;
+                        o[k].z = w ? fmaf(f, v.z, o[k].z) : f * v.z; o[k].w = w ? fmaf(f, v.w, o[k].w) : f * v.w;
+                    }
                 }
+                m = M;
             }
         }
         if (on && sub == 0) {
             const float inv = m == -INFINITY ? 0.f : 1.f / l;      // no token at all: zeros
-            reinterpret_cast<float4 *>(a.out + ((size_t)s * a.Hq + h) * kKvD)[lane] =
-                make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            const int s = row / a.G;
+            float4 *d = reinterpret_cast<float4 *>(a.out + ((size_t)s * a.Hq + (size_t)j * a.G + row - s * a.G) * kKvD) + xq;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                d[4 * k] = make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv);
         }
         return;
     }
@@ -1021,13 +1065,12 @@ __global__ void __launch_bounds__(kJoinWarps * kWarp) kv_join_kernel(const __gri
     const int s = pair / a.Hkv, j = pair % a.Hkv, n = own_len(a, s);
     if (chunk * kJoinWarps * kWarp * 4 >= n) return;
     for (int gq = warp; gq < a.G; gq += kJoinWarps) {
-        const RowPieces x = pieces_of(a, s, j * a.G + gq);
+        const RowPieces x = pieces_of(a, j, s * a.G + gq);
         const int cnt = x.n_pre + x.n_own;
         float m = -INFINITY, l = 0.f;
         for (int i = lane; i < cnt; i += kWarp) {
-            const float *src;
-            const float2 ml = piece_ml(a, x, gq, i, &src);
-            if (src) {
+            const float2 ml = piece_ml(a, x, i);
+            if (ml.x != -INFINITY) {
                 const float mx = fmaxf(m, ml.x);
                 l = (m == -INFINITY ? 0.f : l * ex2(m - mx)) + ml.y * ex2(ml.x - mx);
                 m = mx;
@@ -1202,15 +1245,16 @@ int li_launch_attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_str
     if (a.G <= 8) rc = a.weight ? launch_own<1, true>(a, st) : launch_own<1, false>(a, st);
     else rc = a.weight ? launch_own<2, true>(a, st) : launch_own<2, false>(a, st);
     if (rc) return rc;
-    // warps per row: about 16 records each, going by the most a row can have
+    // warps per 8 rows: as many as it takes to fill the SMs, up to the pieces that a row can have
     const int pairs = a.B * a.Hkv;
     const int64_t pre = a.n_prefix ? 2ll * a.pre_ctas / (a.Hkv * a.n_grp) + 2 : 0;
-    int64_t own = (a.max_ctx + kOwnTok - 1) / kOwnTok / kOwnMinSteps + 2;
+    int64_t own = (a.max_ctx + kOwnTok - 1) / kOwnTok / kOwnMinSteps + 1;
     if (own > a.own_warps / pairs + 2) own = a.own_warps / pairs + 2;
+    const int64_t row_blocks = (int64_t)a.Hkv * ((a.B * a.G + kJoinRows - 1) / kJoinRows);
     a.wpr = 1;
-    while (a.wpr < kJoinWarps && a.wpr * 16 < pre + own) a.wpr *= 2;
+    while (a.wpr < kJoinWarps && a.wpr < pre + own && row_blocks * a.wpr < 16ll * num_sms()) a.wpr *= 2;
     const int per = kJoinWarps / a.wpr;
-    a.row_ctas = (int)(((int64_t)a.B * a.Hq + per - 1) / per);
+    a.row_ctas = (int)((row_blocks + per - 1) / per);
     int64_t blocks = a.row_ctas;
     if (a.weight) {
         const int run = kJoinWarps * kWarp * 4;
