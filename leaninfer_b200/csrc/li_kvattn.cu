@@ -62,13 +62,12 @@ constexpr int kScanMax = 2048;                 // entries of the length scan in 
 
 // ---- prefix part -----------------------------------------------------------
 constexpr int kPreRows = 128, kPreTok = 128;
-constexpr int kPreThreads = 384;               // warps 0-3, 4-7: softmax; 8: TMA; 9: MMA
-constexpr int kPreRegsSoft = 208, kPreRegsRest = 88;        // 256 * 208 + 128 * 88 = 384 * 168
+constexpr int kPreThreads = 512;               // warps 0-3, 4-7: softmax; 8: TMA; 9, 10: MMA; 12-15: records
 constexpr uint32_t kPreSlotBytes = kPreTok * kKvD * 2;      // 128 tokens of K or V: 32 KB
 constexpr uint32_t kPreQBytes = 2 * kPreRows * kKvD * 2;    // a row tile's hi and lo: 64 KB
 constexpr int kPreSlots2 = 3, kPreSlots1 = 5;  // ring slots beside two / one row tiles of q
-constexpr int kPreFlush = 6;                   // token tiles summed in tensor memory before they join the record
-constexpr size_t kPreSmem = 1024 + 2 * kPreQBytes + kPreSlots2 * kPreSlotBytes + 256;
+constexpr int kPreFlush = 4;                   // token tiles summed in tensor memory before they join the record
+constexpr size_t kPreSmem = 1024 + 2 * kPreQBytes + kPreSlots2 * kPreSlotBytes + 256 + 2 * kPreRows * 4;
 static_assert(2 * kPreQBytes + kPreSlots2 * kPreSlotBytes == kPreQBytes + kPreSlots1 * kPreSlotBytes, "ring");
 
 struct KvAttnArgs {
@@ -521,6 +520,11 @@ __device__ __forceinline__ bool softmax_bar_any(bool v) {
 // scores of u + 2, which take the buffer that P of u leaves. So each buffer's
 // softmax runs under the other's products. Tiles, by first use:
 //   nt 2: K0 V0 K1 V1 ...;   nt 1: K0 K1 V0 K2 V1 K3 V2 ...
+// o leaves tensor memory after unit i of a buffer's own count where this holds
+// (and after its last): the two buffers at different times, since both at once
+// would fill the SM's way to L2.
+__device__ __forceinline__ bool sum_ends(int i, int b) { return (i + b * (kPreFlush / 2)) % kPreFlush == kPreFlush - 1; }
+
 __device__ __forceinline__ int k_place(int t, int nt) { return nt == 2 ? 2 * t : t == 0 ? 0 : 2 * t - 1; }
 __device__ __forceinline__ int v_place(int t, int nt, int n) { return nt == 2 ? 2 * t + 1 : t + (t + 2 < n ? t + 2 : n); }
 
@@ -551,15 +555,19 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     uint8_t *ring = smem + (size_t)a.per_group * kPreQBytes;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + 2 * kPreQBytes + kPreSlots2 * kPreSlotBytes);
     uint64_t *full = bars, *empty = full + kPreSlots1, *q_full = empty + kPreSlots1, *s_full = q_full + 1,
-             *p_full = s_full + 2, *o_full = p_full + 4, *turn = o_full + 2, *fin = turn + 2;
-    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(fin + 2);
+             *p_full = s_full + 2, *o_full = p_full + 4, *turn = o_full + 2, *fin = turn + 2, *m_full = fin + 2,
+             *o_read = m_full + 2;
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(o_read + 2);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
+    float *m_of = reinterpret_cast<float *>(bars + 32);            // [buffer][row]: the maximum a sum of P V refers to
     const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
     const int slots = a.slots;
     if (tid == 0) {
         for (int i = 0; i < slots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], a.per_group); }
-        mbar_init(q_full, 8);
+        mbar_init(q_full, 10);
         for (int i = 0; i < 2; ++i) {
+            mbar_init(&m_full[i], 4);
+            mbar_init(&o_read[i], 4);
             mbar_init(&s_full[i], 1);
             mbar_init(&o_full[i], 1);
             mbar_init(&turn[i], 1);
@@ -587,8 +595,69 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     }
     const int p_end = a.Hkv * a.n_grp;
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreRegsRest));
+    if (warp >= 12) {
+        // ---------------- records ----------------
+        // The tensor cores' sums round towards zero, so o is taken out of
+        // tensor memory every kPreFlush units and added, rounded to nearest, to
+        // the record, by warps of its own: only the next sum's first product
+        // waits for it, and that comes after its softmax. A row's words belong
+        // to one thread. (red.global.add.v4.f32 in place of the load and store
+        // was slower by far.)
+        const int r = tid - 384;
+        const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 256u;
+        uint32_t po = 0;                                           // phase of o_full and m_full, a bit per buffer
+        bool ok = true;
+        for (int p = p0; ok && p < p_end; ++p) {
+            const Group g = group_at(a, p);
+            if (g.base >= hi) break;
+            int t0, t1;
+            tiles_of(a, g.base, g.nt, lo, hi, t0, t1);
+            const int n = t1 - t0, U = n * g.nt;
+            float m_rec0 = -INFINITY, m_rec1 = -INFINITY;
+            for (int u = 0; ok && u < U; ++u) {
+                const int b = u & 1;
+                if (u + 2 < U && !sum_ends(u >> 1, b)) continue;
+                const bool live = (g.rt + (g.nt == 2 ? b : 0)) * kPreRows + r < a.rows;
+                float4 *d = reinterpret_cast<float4 *>(a.pre_o + ((size_t)(p + c) * 2 + b) * kPreRows * kKvD) + r;
+                const float m_old = b ? m_rec1 : m_rec0;
+                const bool again = live && m_old != -INFINITY;
+                float4 old[8];
+                auto fetch = [&](int x) {
+#pragma unroll
+                    for (int y = 0; y < 8; ++y)
+                        old[y] = again ? __ldcg(d + (8 * x + y) * kPreRows) : make_float4(0.f, 0.f, 0.f, 0.f);
+                };
+                fetch(0);
+                ok = __all_sync(0xffffffffu, wait_or_abort(&o_full[b], (po >> b) & 1u, abort_flag) &&
+                                                 wait_or_abort(&m_full[b], (po >> b) & 1u, abort_flag));
+                if (!ok) break;
+                po ^= 1u << b;
+                tc_fence_after();
+                const float m = m_of[b * kPreRows + r], f = again ? ex2(m_old - m) : 0.f;
+                (b ? m_rec1 : m_rec0) = m;
+#pragma unroll 1
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t v[32];
+                    tmem_ld32_nowait(lane_base + 128u * b + 32u * x, v);
+                    tmem_wait_ld();
+                    if (x == 3) {                                  // o may be overwritten
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&o_read[b]);
+                    }
+                    if (live)
+#pragma unroll
+                        for (int y = 0; y < 8; ++y)
+                            __stcg(d + (8 * x + y) * kPreRows,
+                                   make_float4(fmaf(old[y].x, f, __uint_as_float(v[4 * y])),
+                                               fmaf(old[y].y, f, __uint_as_float(v[4 * y + 1])),
+                                               fmaf(old[y].z, f, __uint_as_float(v[4 * y + 2])),
+                                               fmaf(old[y].w, f, __uint_as_float(v[4 * y + 3]))));
+                    if (x < 3) fetch(x + 1);
+                }
+            }
+        }
+    } else if (warp >= 8) {
         if (warp == 8 && lane == 0) {
             // ---------------- producer ----------------
             asm volatile("prefetch.tensormap [%0];" ::"l"(&tmK) : "memory");
@@ -641,7 +710,7 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 while (x.slot >= slots) { x.slot -= slots; x.par ^= 1u; }
             };
             int place0 = 0;                                        // ring places before this piece
-            uint32_t pq = 0, pp = 0, pt = 0;                       // phases of q_full, p_full, turn
+            uint32_t pq = 0, pp = 0, pt = 0, pr = 1;               // phases of q_full, p_full, turn, o_read (before)
             bool ok = true, have = b == 0;
             auto acquire = [&]() -> bool {
                 if (!have && !wait_or_abort(&turn[b], pt, abort_flag)) return false;
@@ -659,6 +728,7 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 tiles_of(a, g.base, g.nt, lo, hi, t0, t1);
                 const int n = t1 - t0, U = n * g.nt;
                 if (n <= 0) continue;
+                mbar_arrive(q_full);                               // q_full counts the issuers too: none falls behind
                 if (!(ok = wait_or_abort(q_full, pq, abort_flag))) break;
                 pq ^= 1u;
                 const uint64_t qd = sw128_desc(smem_addr(qbuf) + (g.nt == 2 ? (uint32_t)b * kPreQBytes : 0u));
@@ -666,41 +736,43 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 const int tb = g.nt == 2 ? 0 : b;                  // this buffer's first tile
                 Place kp = place(place0 + k_place(tb, g.nt)), vp = place(place0 + v_place(tb, g.nt, n));
                 place0 += 2 * n;
-                if (b >= U) {                                      // one unit: nothing for buffer 1, but o_full counts
-                    mbar_arrive(&o_full[b]);                       // pieces, so that no issuer falls a piece behind
-                    continue;
-                }
+                if (b >= U) continue;                              // one unit: nothing for buffer 1
                 auto release = [&](int slot) {
                     umma_commit(&empty[slot]);
                     if (g.nt < a.per_group) umma_commit(&empty[slot]);     // for the buffer that does not use it
                 };
                 // scores of unit u; lo first, so that only the hi products add to a sum of full size (the tensor
                 // cores' sums round towards zero, once per instruction)
-                auto scores = [&](uint64_t kd) {
+                auto scores = [&](uint64_t kd, bool turn_over) {
                     tc_fence_after();
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
                         const uint32_t k = 1024u * ((x & 7) >> 2) + 2u * (x & 3);
                         umma_f16(ts, qd + (x < 8 ? 2048u : 0u) + k, kd + k, id_s, x ? 1u : 0u);
+                        if (x == 12 && turn_over) pass();          // the other's first products queue behind the last
                     }
                 };
                 if (!(ok = wait_or_abort(&full[kp.slot], kp.par, abort_flag) && acquire())) break;
-                scores(k0 + (uint64_t)(kp.slot * (kPreSlotBytes >> 4)));
-                if (b == 1 || U > 1) pass();
+                scores(k0 + (uint64_t)(kp.slot * (kPreSlotBytes >> 4)), b == 1 || U > 1);
                 umma_commit(&s_full[b]);
                 release(kp.slot);
                 for (int u = b; u < U; u += 2) {
                     const int t = g.nt == 2 ? u >> 1 : u;
                     const uint64_t vd = v0 + (uint64_t)(vp.slot * (kPreSlotBytes >> 4));
-                    const uint32_t again = (u >> 1) % kPreFlush ? 1u : 0u;
+                    const uint32_t again = u >= 2 && !sum_ends((u >> 1) - 1, b) ? 1u : 0u;
                     const bool more = u + 2 < U;
+                    if (!again) {                                  // a new sum: the last one has been read
+                        if (!(ok = wait_or_abort(&o_read[b], pr, abort_flag))) break;
+                        pr ^= 1u;
+                    }
                     if (!(ok = wait_or_abort(&full[vp.slot], vp.par, abort_flag) &&
                                wait_or_abort(&p_full[2 * b], pp, abort_flag) && acquire()))
                         break;
                     tc_fence_after();
 #pragma unroll
                     for (int x = 0; x < 8; ++x)
-                        umma_f16_ta(to, ts + (x < 4 ? 64u : 0u) + 8u * (x & 3), vd + 128u * (x & 3), id_o, x ? 1u : again);
+                        umma_f16_ta(to, ts + (x < 4 ? 16u : 0u) + 32u * ((x & 3) >> 1) + 8u * (x & 1), vd + 128u * (x & 3),
+                                    id_o, x ? 1u : again);
                     // the first 64 tokens' products run while the softmax ends the other half
                     if (more) {
                         advance(kp, g.nt == 2 ? 2 : k_place(t + 2, 1) - k_place(t, 1));
@@ -711,11 +783,13 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                     tc_fence_after();
 #pragma unroll
                     for (int x = 0; x < 8; ++x)
-                        umma_f16_ta(to, ts + (x < 4 ? 64u : 0u) + 32u + 8u * (x & 3), vd + 512u + 128u * (x & 3), id_o, 1u);
+                        umma_f16_ta(to, ts + 64u + (x < 4 ? 16u : 0u) + 32u * ((x & 3) >> 1) + 8u * (x & 1),
+                                    vd + 512u + 128u * (x & 3), id_o, 1u);
                     // o goes to the record: the buffer's last unit, or kPreFlush of them summed
-                    if (!more || (u >> 1) % kPreFlush == kPreFlush - 1) umma_commit(&o_full[b]);
-                    if (more) scores(k0 + (uint64_t)(kp.slot * (kPreSlotBytes >> 4)));
-                    if (u + 1 < U || b == 1) pass();               // an odd piece ends with buffer 0, which begins the next
+                    if (!more || sum_ends(u >> 1, b)) umma_commit(&o_full[b]);
+                    // an odd piece ends with buffer 0, which begins the next
+                    if (more) scores(k0 + (uint64_t)(kp.slot * (kPreSlotBytes >> 4)), true);
+                    else if (u + 1 < U || b == 1) pass();
                     if (more) umma_commit(&s_full[b]);
                     release(vp.slot);
                     if (more) {
@@ -729,11 +803,10 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         }
     } else {
         // ---------------- softmax: a thread per row of its score buffer ----------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPreRegsSoft));
         const int b = warp >> 2, r = tid & 127;
         const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t sb = lane_base + 128u * b, ob = lane_base + 256u + 128u * b;
-        uint32_t ps = 0, po = 0;                                   // phases of s_full, o_full
+        uint32_t ps = 0, pr = 1;                                   // phases of s_full, o_read (before)
         bool stop = false;
         for (int p = p0; !stop && p < p_end; ++p) {
             const Group g = group_at(a, p);
@@ -742,80 +815,62 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             tiles_of(a, g.base, g.nt, lo, hi, t0, t1);
             const int n = t1 - t0;
             if (n <= 0) continue;
-            // this row's q: scaled, split and stored as the operand's rows
-            const int row = (g.rt + (g.nt == 2 ? b : 0)) * kPreRows + r;
+            // this warp's 32 rows of q: scaled, split and stored as the operand's rows. A warp reads a row at a
+            // time (512 contiguous bytes; a thread per row took 20,000 cycles), lane l its dims 4l .. 4l+3.
+            const int tile0 = (g.rt + (g.nt == 2 ? b : 0)) * kPreRows, row = tile0 + r;
             const bool live = row < a.rows;
-            float c2;
+            float c2 = 0.f;
             {
-                const int s = live ? row / a.G : 0, h = live ? g.j * a.G + row - s * a.G : 0;
-                const float4 *qs = reinterpret_cast<const float4 *>(a.q + s * a.q_stride + (size_t)h * kKvD);
-                float4 x[32];
-                float mx = 0.f;
+                uint8_t *qd = qbuf + (g.nt == 2 ? (size_t)b * kPreQBytes : 0) + (lane >> 4) * 16384 + (lane & 1) * 8;
+                const bool put = g.nt == 2 || b == 0;
+                int rr = tile0 + 32 * (warp & 3), s = rr / a.G, h = rr - s * a.G;      // the next row to fetch
+                float4 x[4];
+                auto fetch = [&](float4 (&v)[4]) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    x[i] = live ? __ldcg(qs + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
-                }
-                const float p2 = pow2_of(mx), inv = inv_pow2(p2) * a.qsign;
-                c2 = fmaxf(a.cscale * p2, 1.17549435e-38f);        // not 0: a masked score is -inf c2
-                if (g.nt == 2 || b == 0) {
-                    uint8_t *qd = qbuf + (g.nt == 2 ? (size_t)b * kPreQBytes : 0);
+                    for (int i = 0; i < 4; ++i) {
+                        v[i] = rr < a.rows ? __ldcg(reinterpret_cast<const float4 *>(
+                                                        a.q + s * a.q_stride + (size_t)(g.j * a.G + h) * kKvD) + lane)
+                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+                        ++rr;
+                        if (++h == a.G) { h = 0; ++s; }
+                    }
+                };
+                fetch(x);
+                // loops stay rolled here: code that runs once per piece costs its instruction fetches
+#pragma unroll 1
+                for (int r0 = 0; r0 < 32; r0 += 4) {
+                    float4 v[4];
+                    float mx[4];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float y[8] = {x[2 * i].x * inv, x[2 * i].y * inv, x[2 * i].z * inv, x[2 * i].w * inv,
-                                            x[2 * i + 1].x * inv, x[2 * i + 1].y * inv, x[2 * i + 1].z * inv,
-                                            x[2 * i + 1].w * inv};
-                        uint32_t hw[4], lw[4];
+                    for (int i = 0; i < 4; ++i) {
+                        v[i] = x[i];
+                        mx[i] = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+                    }
+                    if (r0 < 28) fetch(x);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float h0 = hi_part(y[2 * e]), h1 = hi_part(y[2 * e + 1]);
-                            hw[e] = pack_h2(h0, h1);
-                            lw[e] = pack_h2(y[2 * e] - h0, y[2 * e + 1] - h1);
+                    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p2 = pow2_of(mx[i]), inv = inv_pow2(p2) * a.qsign;
+                        if (lane == r0 + i) c2 = fmaxf(a.cscale * p2, 1.17549435e-38f);   // not 0: a masked score is -inf c2
+                        const float y[4] = {v[i].x * inv, v[i].y * inv, v[i].z * inv, v[i].w * inv};
+                        const float h4[4] = {hi_part(y[0]), hi_part(y[1]), hi_part(y[2]), hi_part(y[3])};
+                        const uint32_t off = sw128_off(32 * (warp & 3) + r0 + i, (lane & 15) >> 1);
+                        if (put) {
+                            *reinterpret_cast<uint2 *>(qd + off) = make_uint2(pack_h2(h4[0], h4[1]), pack_h2(h4[2], h4[3]));
+                            *reinterpret_cast<uint2 *>(qd + 32768 + off) =
+                                make_uint2(pack_h2(y[0] - h4[0], y[1] - h4[1]), pack_h2(y[2] - h4[2], y[3] - h4[3]));
                         }
-                        const uint32_t off = (uint32_t)(i >> 3) * 16384u + sw128_off(r, i & 7);
-                        *reinterpret_cast<uint4 *>(qd + off) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-                        *reinterpret_cast<uint4 *>(qd + 32768 + off) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
                     }
                 }
             }
             fence_proxy_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
-            float m = -INFINITY, l = 0.f, m_rec = -INFINITY;
+            float m = -INFINITY, l = 0.f;
             bool ok = true;
-            const size_t rec = ((size_t)(p + c) * 2 + b) * kPreRows;
-            float4 *d = reinterpret_cast<float4 *>(a.pre_o + rec * kKvD) + r;      // [32 groups of 4 dims][128 rows]
-            // o in tensor memory joins this row of the record, whose values have the factor 2^(m_rec); the record's
-            // old values are fetched while the products run
-            auto flush = [&]() -> bool {
-                float4 old[32];
-                const bool again = m_rec != -INFINITY;
-                const float fr = again ? ex2(m_rec - m) : 0.f;
-#pragma unroll
-                for (int x = 0; x < 32; ++x) old[x] = again && live ? __ldcg(d + x * kPreRows) : make_float4(0.f, 0.f, 0.f, 0.f);
-                if (!__all_sync(0xffffffffu, wait_or_abort(&o_full[b], po, abort_flag))) return false;
-                po ^= 1u;
-                tc_fence_after();
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    uint32_t ov[32];
-                    tmem_ld32_nowait(ob + 32u * x, ov);
-                    tmem_wait_ld();
-                    if (live)
-#pragma unroll
-                        for (int y = 0; y < 8; ++y) {
-                            const float4 w = old[8 * x + y];
-                            __stcg(d + (8 * x + y) * kPreRows,
-                                   make_float4(fmaf(w.x, fr, __uint_as_float(ov[4 * y])),
-                                               fmaf(w.y, fr, __uint_as_float(ov[4 * y + 1])),
-                                               fmaf(w.z, fr, __uint_as_float(ov[4 * y + 2])),
-                                               fmaf(w.w, fr, __uint_as_float(ov[4 * y + 3]))));
-                        }
-                }
-                tc_fence_before();
-                m_rec = m;
-                return true;
-            };
             int unit = 0;
             // this buffer's token tiles: every one (nt 2), or every second one
             const int first = g.nt == 2 ? 0 : b, step = g.nt == 2 ? 1 : 2;
@@ -824,37 +879,35 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 if (!ok) break;
                 ps ^= 1u;
                 tc_fence_after();
-                uint32_t v[4][32];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) tmem_ld32_nowait(sb + 32u * x, v[x]);
-                tmem_wait_ld();
+                // The scores are read twice, 32 tokens at a time, so that few are held in registers: for their
+                // maximum, then for P, whose hi and lo parts (16 columns each) take the place of the 32 scores.
                 const int left = a.n_prefix - (t0 + i) * kPreTok;
-                if (left < kPreTok) {
+                float mx;
+                {
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                    for (int x = 0; x < kPreTok && x < left; x += 32) {
+                        uint32_t v[32];
+                        tmem_ld32_nowait(sb + (uint32_t)x, v);
+                        tmem_wait_ld();
+                        if (left - x < 32) {
 #pragma unroll
-                    for (int x = 0; x < 128; ++x)
-                        if (x >= left) v[x >> 5][x & 31] = 0xff800000u;            // -inf
-                }
-                float m8[8];
+                            for (int y = 0; y < 32; ++y)
+                                if (x + y >= left) v[y] = 0xff800000u;     // -inf
+                        }
 #pragma unroll
-                for (int x = 0; x < 8; ++x)
-                    m8[x] = fmaxf(__uint_as_float(v[0][x]), fmaxf(__uint_as_float(v[0][8 + x]),
-                                                                  __uint_as_float(v[0][16 + x])));
+                        for (int y = 0; y < 32; y += 8)
 #pragma unroll
-                for (int y = 24; y < 120; y += 16)
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        const int e = y + x, f = y + 8 + x;
-                        m8[x] = fmaxf(m8[x], fmaxf(__uint_as_float(v[e >> 5][e & 31]), __uint_as_float(v[f >> 5][f & 31])));
+                            for (int e = 0; e < 4; ++e)
+                                m4[e] = fmaxf(m4[e], fmaxf(__uint_as_float(v[y + e]), __uint_as_float(v[y + 4 + e])));
                     }
-#pragma unroll
-                for (int x = 0; x < 8; ++x) m8[x] = fmaxf(m8[x], __uint_as_float(v[3][24 + x]));
-                const float mx = c2 * fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
-                                            fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
+                    mx = c2 * fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                }
                 const bool grow = mx > m + kMaxLag;
                 const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2(m - mx);
                 if (grow) m = mx;
                 l *= f;
-                if (unit % kPreFlush && __any_sync(0xffffffffu, grow)) {
+                if (unit > 0 && !sum_ends(unit - 1, b) && __any_sync(0xffffffffu, grow)) {
                     // P V of this buffer's last tile is complete: these scores were issued after it
                     for (int x = 0; x < 4; ++x) {
                         uint32_t ov[32];
@@ -866,48 +919,54 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                     }
                 }
                 const uint64_t cc = pack2(c2, c2), off = pack2(kPShift - m, kPShift - m), minus = pack2(-1.f, -1.f);
-                uint64_t ls[4] = {0, 0, 0, 0};
+                uint64_t ls[2] = {0, 0};
+#pragma unroll 1
+                for (int x = 0; x < kPreTok; x += 32) {
+                    uint32_t v[32], w[32];
+                    tmem_ld32_nowait(sb + (uint32_t)x, v);
+                    tmem_wait_ld();
+                    if (left - x < 32) {
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    uint32_t hw[32], lw[32];
+                        for (int y = 0; y < 32; ++y)
+                            if (x + y >= left) v[y] = 0xff800000u;
+                    }
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) {
-                        const int e = 64 * hf + 2 * x;
+                    for (int y = 0; y < 16; ++y) {
                         float p0, p1, d0, d1;
-                        unpack2(fma2(pack2(__uint_as_float(v[e >> 5][e & 31]), __uint_as_float(v[e >> 5][(e & 31) + 1])),
-                                     cc, off), p0, p1);
+                        unpack2(fma2(pack2(__uint_as_float(v[2 * y]), __uint_as_float(v[2 * y + 1])), cc, off), p0, p1);
                         p0 = ex2(p0);
                         p1 = ex2(p1);
                         const uint64_t pp = pack2(p0, p1);
-                        ls[x & 3] = add2(ls[x & 3], pp);
+                        ls[y & 1] = add2(ls[y & 1], pp);
                         const float h0 = hi_part(p0), h1 = hi_part(p1);
-                        hw[x] = pack_h2(h0, h1);
+                        w[y] = pack_h2(h0, h1);
                         unpack2(fma2(pack2(h0, h1), minus, pp), d0, d1);
-                        lw[x] = pack_h2(d0, d1);
+                        w[16 + y] = pack_h2(d0, d1);
                     }
-                    tmem_st32(sb + 32u * hf, hw);
-                    tmem_st32(sb + 64u + 32u * hf, lw);
-                    tmem_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[2 * b + hf]);
+                    tmem_st32(sb + (uint32_t)x, w);
+                    if (x & 32) {                                  // 64 tokens: their products may begin
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_full[2 * b + (x >> 6)]);
+                    }
                 }
                 {
                     float l0, l1;
-                    unpack2(add2(add2(ls[0], ls[1]), add2(ls[2], ls[3])), l0, l1);
+                    unpack2(add2(ls[0], ls[1]), l0, l1);
                     l += l0 + l1;
                 }
-                // P V of this unit ends a sum: the buffer's last, or kPreFlush of them
-                if (i + step >= n || unit % kPreFlush == kPreFlush - 1) {
-                    ok = flush();
+                // P V of this unit ends a sum: the maximum it refers to, once the last sum's has been read
+                if (i + step >= n || sum_ends(unit, b)) {
+                    ok = __all_sync(0xffffffffu, wait_or_abort(&o_read[b], pr, abort_flag));
                     if (!ok) break;
+                    pr ^= 1u;
+                    m_of[b * kPreRows + r] = m;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&m_full[b]);
                 }
             }
-            if (ok && first >= n) {
-                ok = __all_sync(0xffffffffu, wait_or_abort(&o_full[b], po, abort_flag));
-                po ^= 1u;
-            }
-            if (ok && live && first < n) a.pre_ml[rec + r] = make_float2(m - kPShift, l);
+            if (ok && live && first < n) a.pre_ml[((size_t)(p + c) * 2 + b) * kPreRows + r] = make_float2(m - kPShift, l);
             // both buffers are done with q before the next piece's is written
             stop = softmax_bar_any(!ok);
         }
@@ -1005,28 +1064,50 @@ __global__ void __launch_bounds__(kJoinWarps * kWarp) kv_join_kernel(const __gri
         if (on) {
             const RowPieces x = pieces_of(a, j, row);
             const int n = x.n_pre + x.n_own;
-            for (int i = sub; i < n; i += a.wpr) m = fmaxf(m, piece_ml(a, x, i).x);
-#pragma unroll 2
-            for (int i = sub; i < n; i += a.wpr) {
-                const float2 ml = piece_ml(a, x, i);
-                const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
-                l = fmaf(f, ml.y, l);
-                const float4 *src = nullptr;
-                int step = 0;
-                if (i >= x.n_pre) {
-                    src = reinterpret_cast<const float4 *>(a.own_o + ((size_t)(x.rec0 + i - x.n_pre) * a.G + x.gq) * kKvD) + xq;
-                    step = 4;
-                } else if (const int rec = pre_record(a, x, i); rec >= 0) {
-                    src = reinterpret_cast<const float4 *>(a.pre_o) + ((size_t)rec * 32 + xq) * kPreRows + x.prow;
-                    step = 4 * kPreRows;
-                }
-                if (src)
+            // four pieces at a time, their loads in flight together (predicated, not branched over)
+            for (int i0 = sub; i0 < n; i0 += 4 * a.wpr) {
+                const float4 *src[4];
+                int step[4];
+                float2 ml[4];
+                float mx = m;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float4 v = __ldcg(src + k * step);
-                        o[k].x = fmaf(f, v.x, o[k].x); o[k].y = fmaf(f, v.y, o[k].y);
-                        o[k].z = fmaf(f, v.z, o[k].z); o[k].w = fmaf(f, v.w, o[k].w);
+                for (int k = 0; k < 4; ++k) {
+                    const int i = i0 + k * a.wpr;
+                    const bool pre = i < x.n_pre;
+                    const int rec = i >= n ? -1 : pre ? pre_record(a, x, i) : (x.rec0 + i - x.n_pre) * a.G + x.gq;
+                    src[k] = rec < 0 ? nullptr
+                             : pre   ? reinterpret_cast<const float4 *>(a.pre_o) + ((size_t)rec * 32 + xq) * kPreRows + x.prow
+                                     : reinterpret_cast<const float4 *>(a.own_o) + (size_t)rec * 32 + xq;
+                    step[k] = pre ? 4 * kPreRows : 4;
+                    const float2 *mp = pre ? a.pre_ml + (size_t)max(rec, 0) * kPreRows + x.prow : a.own_ml + max(rec, 0);
+                    ml[k] = rec >= 0 ? __ldcg(mp) : make_float2(-INFINITY, 0.f);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mx = fmaxf(mx, ml[k].x);
+                const float keep = m == -INFINITY ? 0.f : ex2(m - mx);
+                m = mx;
+                l *= keep;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) { o[k].x *= keep; o[k].y *= keep; o[k].z *= keep; o[k].w *= keep; }
+#pragma unroll
+                for (int h = 0; h < 4; h += 2) {
+                    float4 v[2][8];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            v[e][k] = src[h + e] ? __ldcg(src[h + e] + k * step[h + e]) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float f = src[h + e] ? ex2(ml[h + e].x - m) : 0.f;
+                        l = fmaf(f, ml[h + e].y, l);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            o[k].x = fmaf(f, v[e][k].x, o[k].x); o[k].y = fmaf(f, v[e][k].y, o[k].y);
+                            o[k].z = fmaf(f, v[e][k].z, o[k].z); o[k].w = fmaf(f, v[e][k].w, o[k].w);
+                        }
                     }
+                }
             }
         }
         if (a.wpr > 1) {
