@@ -93,7 +93,7 @@ struct KvAttnArgs {
     float2 *pre_ml;                    // [Hkv n_grp + pre_ctas][2][128 rows]
     float *pre_o;                      // [Hkv n_grp + pre_ctas][2][32 groups of 4 dims][128 rows][4]
     // join
-    int row_ctas, wpr, w_chunks;       // blocks that join rows, warps per 8 rows, blocks per pair that write weights
+    int row_ctas, wpr, w_chunks;       // blocks that join rows, warps per 4 rows, blocks per pair that write weights
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -815,56 +815,60 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             tiles_of(a, g.base, g.nt, lo, hi, t0, t1);
             const int n = t1 - t0;
             if (n <= 0) continue;
-            // this warp's 32 rows of q: scaled, split and stored as the operand's rows. A warp reads a row at a
-            // time (512 contiguous bytes; a thread per row took 20,000 cycles), lane l its dims 4l .. 4l+3.
+            // this warp's 32 rows of q: scaled, split and stored as the operand's rows. Eight lanes take a row
+            // (128 contiguous bytes a load), four rows a step, two steps' loads in flight.
             const int tile0 = (g.rt + (g.nt == 2 ? b : 0)) * kPreRows, row = tile0 + r;
             const bool live = row < a.rows;
             float c2 = 0.f;
             {
-                uint8_t *qd = qbuf + (g.nt == 2 ? (size_t)b * kPreQBytes : 0) + (lane >> 4) * 16384 + (lane & 1) * 8;
+                const int sub = lane >> 3, l8 = lane & 7;
                 const bool put = g.nt == 2 || b == 0;
-                int rr = tile0 + 32 * (warp & 3), s = rr / a.G, h = rr - s * a.G;      // the next row to fetch
-                float4 x[4];
+                uint8_t *qd = qbuf + (g.nt == 2 ? (size_t)b * kPreQBytes : 0) + (l8 & 1) * 8;
+                int rr = tile0 + 32 * (warp & 3) + sub, s = rr / a.G, h = rr - s * a.G;      // the row to fetch next
+                float4 x[2][4];
                 auto fetch = [&](float4 (&v)[4]) {
+                    const float4 *src = reinterpret_cast<const float4 *>(a.q + s * a.q_stride + (size_t)(g.j * a.G + h) * kKvD) + l8;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        v[i] = rr < a.rows ? __ldcg(reinterpret_cast<const float4 *>(
-                                                        a.q + s * a.q_stride + (size_t)(g.j * a.G + h) * kKvD) + lane)
-                                           : make_float4(0.f, 0.f, 0.f, 0.f);
-                        ++rr;
-                        if (++h == a.G) { h = 0; ++s; }
-                    }
+                    for (int k = 0; k < 4; ++k)
+                        v[k] = rr < a.rows ? __ldcg(src + 8 * k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    rr += 4;
+                    h += 4;
+                    while (h >= a.G) { h -= a.G; ++s; }
                 };
-                fetch(x);
-                // loops stay rolled here: code that runs once per piece costs its instruction fetches
+#pragma unroll
+                for (int i = 0; i < 2; ++i) fetch(x[i]);
+                // rolled: code that runs once a piece costs its instruction fetches
 #pragma unroll 1
-                for (int r0 = 0; r0 < 32; r0 += 4) {
-                    float4 v[4];
-                    float mx[4];
+                for (int i0 = 0; i0 < 8; i0 += 2)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        v[i] = x[i];
-                        mx[i] = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
-                    }
-                    if (r0 < 28) fetch(x);
+                    for (int i = 0; i < 2; ++i) {
+                        float4 v[4];
+                        float mx = 0.f;
 #pragma unroll
-                    for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p2 = pow2_of(mx[i]), inv = inv_pow2(p2) * a.qsign;
-                        if (lane == r0 + i) c2 = fmaxf(a.cscale * p2, 1.17549435e-38f);   // not 0: a masked score is -inf c2
-                        const float y[4] = {v[i].x * inv, v[i].y * inv, v[i].z * inv, v[i].w * inv};
-                        const float h4[4] = {hi_part(y[0]), hi_part(y[1]), hi_part(y[2]), hi_part(y[3])};
-                        const uint32_t off = sw128_off(32 * (warp & 3) + r0 + i, (lane & 15) >> 1);
-                        if (put) {
-                            *reinterpret_cast<uint2 *>(qd + off) = make_uint2(pack_h2(h4[0], h4[1]), pack_h2(h4[2], h4[3]));
-                            *reinterpret_cast<uint2 *>(qd + 32768 + off) =
-                                make_uint2(pack_h2(y[0] - h4[0], y[1] - h4[1]), pack_h2(y[2] - h4[2], y[3] - h4[3]));
+                        for (int k = 0; k < 4; ++k) {
+                            v[k] = x[i][k];
+                            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
                         }
+                        if (i0 < 6) fetch(x[i]);
+#pragma unroll
+                        for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        const float p2 = pow2_of(mx), inv = inv_pow2(p2) * a.qsign;
+                        const float mine = __shfl_sync(0xffffffffu, p2, (lane & 3) * 8);
+                        if (lane >> 2 == i0 + i) c2 = fmaxf(a.cscale * mine, 1.17549435e-38f);   // not 0: a masked score is -inf c2
+                        const int rt = 32 * (warp & 3) + 4 * (i0 + i) + sub;                    // row of the tile
+                        if (put)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float y[4] = {v[k].x * inv, v[k].y * inv, v[k].z * inv, v[k].w * inv};
+                                const float h4[4] = {hi_part(y[0]), hi_part(y[1]), hi_part(y[2]), hi_part(y[3])};
+                                // dims 32 k + 4 l8 ..: 16-byte granule 4 k + l8 / 2 of the row, 8 granules a block
+                                const uint32_t off = (uint32_t)(k >> 1) * 16384u + sw128_off(rt, 4 * (k & 1) + (l8 >> 1));
+                                *reinterpret_cast<uint2 *>(qd + off) =
+                                    make_uint2(pack_h2(h4[0], h4[1]), pack_h2(h4[2], h4[3]));
+                                *reinterpret_cast<uint2 *>(qd + 32768 + off) =
+                                    make_uint2(pack_h2(y[0] - h4[0], y[1] - h4[1]), pack_h2(y[2] - h4[2], y[3] - h4[3]));
+                            }
                     }
-                }
             }
             fence_proxy_async_shared();
             __syncwarp();
@@ -1039,14 +1043,14 @@ __device__ __forceinline__ float2 piece_ml(const KvAttnArgs &a, const RowPieces 
     return __ldcg(a.own_ml + (size_t)(x.rec0 + i - x.n_pre) * a.G + x.gq);
 }
 
-constexpr int kJoinWarps = 8, kJoinRows = 8;
+constexpr int kJoinWarps = 8, kJoinRows = 4;
 
-// Rows: wpr neighbouring warps take 8 rows of a kv head, each its share of the
-// pieces; lane l holds row l % 8 and dims 16 i + 4 (l / 8) .. +3, i < 8, so that
-// a load reads 128 contiguous bytes of each of four dim groups.
-__global__ void __launch_bounds__(kJoinWarps * kWarp) kv_join_kernel(const __grid_constant__ KvAttnArgs a) {
+// Rows: wpr neighbouring warps take 4 rows of a kv head, each its share of the
+// pieces; lane l holds row l % 4 and dims 32 i + 4 (l / 4) .. +3, i < 4 (the
+// prefix's records lie dims first, so a load reads whole sectors either way).
+__global__ void __launch_bounds__(kJoinWarps * kWarp, 3) kv_join_kernel(const __grid_constant__ KvAttnArgs a) {
     __shared__ float red_m[kJoinWarps][kJoinRows], red_l[kJoinWarps][kJoinRows];
-    __shared__ __align__(16) float4 red_o[kJoinWarps][8][kWarp];
+    __shared__ __align__(16) float4 red_o[kJoinWarps][4][kWarp];
     __shared__ float gm[16], gi[16];
     grid_dep_wait();
     grid_dep_launch_dependents();
@@ -1055,65 +1059,54 @@ __global__ void __launch_bounds__(kJoinWarps * kWarp) kv_join_kernel(const __gri
         const int per = kJoinWarps / a.wpr, sub = warp % a.wpr;
         const int rows = a.B * a.G, blocks = (rows + kJoinRows - 1) / kJoinRows;      // row blocks of a kv head
         const int item = blockIdx.x * per + warp / a.wpr, j = item / blocks;
-        const int rl = lane & 7, xq = lane >> 3, row = (item - j * blocks) * kJoinRows + rl;
+        const int rl = lane & 3, xq = lane >> 2, row = (item - j * blocks) * kJoinRows + rl;
         const bool on = j < a.Hkv && row < rows;
         float m = -INFINITY, l = 0.f;
-        float4 o[8];
+        float4 o[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (on) {
             const RowPieces x = pieces_of(a, j, row);
             const int n = x.n_pre + x.n_own;
-            // four pieces at a time, their loads in flight together (predicated, not branched over)
-            for (int i0 = sub; i0 < n; i0 += 4 * a.wpr) {
-                const float4 *src[4];
-                int step[4];
-                float2 ml[4];
-                float mx = m;
+            // two pieces at a time, their loads in flight together (predicated, not branched over)
+            for (int i0 = sub; i0 < n; i0 += 2 * a.wpr) {
+                float4 v[2][4];
+                float2 ml[2];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int i = i0 + k * a.wpr;
+                for (int e = 0; e < 2; ++e) {
+                    const int i = i0 + e * a.wpr;
                     const bool pre = i < x.n_pre;
                     const int rec = i >= n ? -1 : pre ? pre_record(a, x, i) : (x.rec0 + i - x.n_pre) * a.G + x.gq;
-                    src[k] = rec < 0 ? nullptr
-                             : pre   ? reinterpret_cast<const float4 *>(a.pre_o) + ((size_t)rec * 32 + xq) * kPreRows + x.prow
-                                     : reinterpret_cast<const float4 *>(a.own_o) + (size_t)rec * 32 + xq;
-                    step[k] = pre ? 4 * kPreRows : 4;
+                    const float4 *src = pre ? reinterpret_cast<const float4 *>(a.pre_o) +
+                                                  ((size_t)max(rec, 0) * 32 + xq) * kPreRows + x.prow
+                                            : reinterpret_cast<const float4 *>(a.own_o) + (size_t)max(rec, 0) * 32 + xq;
                     const float2 *mp = pre ? a.pre_ml + (size_t)max(rec, 0) * kPreRows + x.prow : a.own_ml + max(rec, 0);
-                    ml[k] = rec >= 0 ? __ldcg(mp) : make_float2(-INFINITY, 0.f);
+                    const int step = pre ? 8 * kPreRows : 8;
+                    ml[e] = rec >= 0 ? __ldcg(mp) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        v[e][k] = rec >= 0 ? __ldcg(src + k * step) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) mx = fmaxf(mx, ml[k].x);
+                const float mx = fmaxf(m, fmaxf(ml[0].x, ml[1].x));
                 const float keep = m == -INFINITY ? 0.f : ex2(m - mx);
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) f[e] = ml[e].x == -INFINITY ? 0.f : ex2(ml[e].x - mx);
                 m = mx;
-                l *= keep;
+                l = fmaf(f[0], ml[0].y, fmaf(f[1], ml[1].y, l * keep));
 #pragma unroll
-                for (int k = 0; k < 8; ++k) { o[k].x *= keep; o[k].y *= keep; o[k].z *= keep; o[k].w *= keep; }
-#pragma unroll
-                for (int h = 0; h < 4; h += 2) {
-                    float4 v[2][8];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            v[e][k] = src[h + e] ? __ldcg(src[h + e] + k * step[h + e]) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float f = src[h + e] ? ex2(ml[h + e].x - m) : 0.f;
-                        l = fmaf(f, ml[h + e].y, l);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            o[k].x = fmaf(f, v[e][k].x, o[k].x); o[k].y = fmaf(f, v[e][k].y, o[k].y);
-                            o[k].z = fmaf(f, v[e][k].z, o[k].z); o[k].w = fmaf(f, v[e][k].w, o[k].w);
-                        }
-                    }
+                for (int k = 0; k < 4; ++k) {
+                    o[k].x = fmaf(f[0], v[0][k].x, fmaf(f[1], v[1][k].x, o[k].x * keep));
+                    o[k].y = fmaf(f[0], v[0][k].y, fmaf(f[1], v[1][k].y, o[k].y * keep));
+                    o[k].z = fmaf(f[0], v[0][k].z, fmaf(f[1], v[1][k].z, o[k].z * keep));
+                    o[k].w = fmaf(f[0], v[0][k].w, fmaf(f[1], v[1][k].w, o[k].w * keep));
                 }
             }
         }
         if (a.wpr > 1) {
             if (xq == 0) { red_m[warp][rl] = m; red_l[warp][rl] = l; }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) red_o[warp][k][lane] = o[k];
+            for (int k = 0; k < 4; ++k) red_o[warp][k][lane] = o[k];
             __syncthreads();
             if (sub == 0) {
                 float M = m;
@@ -1122,7 +1115,7 @@ __global__ void __launch_bounds__(kJoinWarps * kWarp) kv_join_kernel(const __gri
                     const float f = red_m[warp + w][rl] == -INFINITY ? 0.f : ex2(red_m[warp + w][rl] - M);
                     l = w ? fmaf(f, red_l[warp + w][rl], l) : f * l;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
+                    for (int k = 0; k < 4; ++k) {
                         const float4 v = red_o[warp + w][k][lane];
                         o[k].x = w ? fmaf(f, v.x, o[k].x) : f * v.x; o[k].y = w ? fmaf(f, v.y, o[k].y) : f * v.y;
                         o[k].z = w ? fmaf(f, v.z, o[k].z) : f * v.z; o[k].w = w ? fmaf(f, v.w, o[k].w) : f * v.w;
@@ -1136,8 +1129,8 @@ __global__ void __launch_bounds__(kJoinWarps * kWarp) kv_join_kernel(const __gri
             const int s = row / a.G;
             float4 *d = reinterpret_cast<float4 *>(a.out + ((size_t)s * a.Hq + (size_t)j * a.G + row - s * a.G) * kKvD) + xq;
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                d[4 * k] = make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv);
+            for (int k = 0; k < 4; ++k)
+                d[8 * k] = make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv);
         }
         return;
     }
@@ -1326,7 +1319,7 @@ int li_launch_attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_str
     if (a.G <= 8) rc = a.weight ? launch_own<1, true>(a, st) : launch_own<1, false>(a, st);
     else rc = a.weight ? launch_own<2, true>(a, st) : launch_own<2, false>(a, st);
     if (rc) return rc;
-    // warps per 8 rows: as many as it takes to fill the SMs, up to the pieces that a row can have
+    // warps per 4 rows: as many as it takes to fill the SMs, up to the pieces that a row can have
     const int pairs = a.B * a.Hkv;
     const int64_t pre = a.n_prefix ? 2ll * a.pre_ctas / (a.Hkv * a.n_grp) + 2 : 0;
     int64_t own = (a.max_ctx + kOwnTok - 1) / kOwnTok / kOwnMinSteps + 1;
