@@ -10,10 +10,14 @@
 // all moves are independent and need no order.
 //
 //   kv_select   block per (sequence, kv head): the budget-th largest key by a
-//               radix search over four 8-bit digits, then the two ascending
-//               lists by warp ballots and a block scan;
-//   kv_move     warps over all lists: 512 bytes (K and V row) per move, plus
-//               weight and position.
+//               radix search over digits of 11, 11 and 10 bits, the two
+//               ascending lists by warp ballots and a block scan, and the first
+//               kSelMoves moves themselves: 512 bytes (K and V row) each, plus
+//               weight and position, eight a warp in flight. That is all there
+//               is where a cache overshoots its budget by a little, as it does
+//               in use;
+//   kv_move     the moves beyond those, warps over all lists, and the lengths
+//               (which every block of kv_select reads).
 #include "li_kv.cuh"
 
 LI_DEFINE_TU_STATUS(kvevict)
@@ -21,9 +25,11 @@ LI_DEFINE_TU_STATUS(kvevict)
 namespace li {
 namespace {
 
-constexpr int kSelThreads = 512;
-constexpr int kSelWarps = kSelThreads / kWarp;
 constexpr int kSelCacheMax = 48 * 1024;     // keys held in shared memory up to this many slots
+constexpr int kSelWide = 8192;              // from this many slots on, blocks of 1024 threads
+constexpr int kSelMoves = 256;              // moves that kv_select makes itself
+constexpr int kBins = 2048;                 // of a digit
+constexpr int kMovePer = 8;                 // moves of a warp in flight
 
 struct EvictArgs {
     const float *weight;
@@ -46,6 +52,7 @@ __device__ __forceinline__ uint32_t evict_key(float w, int p, int64_t first_free
 
 // Exclusive scan of v over the block's warps (one value per warp, given by
 // every lane); returns this warp's offset and the total.
+template <int W>
 __device__ __forceinline__ int warp_offsets(int v, int *buf, int &total) {
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     __syncthreads();
@@ -53,7 +60,7 @@ __device__ __forceinline__ int warp_offsets(int v, int *buf, int &total) {
     __syncthreads();
     int off = 0, sum = 0;
 #pragma unroll
-    for (int w = 0; w < kSelWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
         const int x = buf[w];
         if (w < warp) off += x;
         sum += x;
@@ -62,12 +69,32 @@ __device__ __forceinline__ int warp_offsets(int v, int *buf, int &total) {
     return off;
 }
 
-__global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictArgs a, bool cached) {
+// Rows m, m + stride, ... of a pair's moves: lanes 0-15 carry the K row, 16-31
+// the V row, 16 bytes each; the loads of kMovePer rows go out together.
+template <typename List>
+__device__ __forceinline__ void move_rows(const EvictArgs &a, int pair, List move, int m, int n, int stride, int lane) {
+    const int s = pair / a.Hkv, j = pair - s * a.Hkv;
+    __half *base = (lane < 16 ? a.k : a.v) + ((size_t)s * a.max_ctx * a.Hkv + j) * kKvD + (lane & 15) * 8;
+    const size_t row = (size_t)a.Hkv * kKvD;
+    for (; m < n; m += kMovePer * stride) {
+        uint4 d[kMovePer];
+#pragma unroll
+        for (int i = 0; i < kMovePer; ++i)
+            if (m + i * stride < n) d[i] = *reinterpret_cast<const uint4 *>(base + (size_t)move(m + i * stride).x * row);
+#pragma unroll
+        for (int i = 0; i < kMovePer; ++i)
+            if (m + i * stride < n) *reinterpret_cast<uint4 *>(base + (size_t)move(m + i * stride).y * row) = d[i];
+    }
+}
+
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) kv_select_kernel(EvictArgs a, bool cached) {
+    constexpr int W = THREADS / kWarp, kPer = kBins / THREADS;
     extern __shared__ uint32_t keys[];             // [max_ctx] when cached
-    __shared__ int hist[256];
-    __shared__ int buf[kSelWarps];
-    __shared__ uint32_t s_digit;
-    __shared__ int s_want;
+    __shared__ int hist[kBins];
+    __shared__ int buf[W];
+    __shared__ int s_digit, s_want;
+    __shared__ int2 mine[kSelMoves];
     grid_dep_wait();
     grid_dep_launch_dependents();
     const int pair = blockIdx.x, s = pair / a.Hkv;
@@ -90,36 +117,54 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictArgs a, boo
     auto key_of = [&](int i) -> uint32_t {
         return cached ? keys[i] : evict_key(w[i], sp[i], a.first_free, newest_free);
     };
-    if (cached)
-        for (int i = tid; i < n; i += kSelThreads) keys[i] = evict_key(w[i], sp[i], a.first_free, newest_free);
-
+    if (cached) {
+#pragma unroll 4
+        for (int i = tid; i < n; i += THREADS) keys[i] = evict_key(w[i], sp[i], a.first_free, newest_free);
+    }
     // the budget-th largest key, digit by digit from the top: `prefix` holds
     // the digits found, `want` the rank left among the keys that share them
     uint32_t prefix = 0, mask = 0;
     int want = a.budget;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t digits = pass == 2 ? 1023u : 2047u;
+        for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += kSelThreads) {
+        for (int i = tid; i < n; i += THREADS) {
             const uint32_t k = key_of(i);
-            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1);
+            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digits], 1);
         }
         __syncthreads();
-        if (tid == 0) {
-            int left = want, d = 255;
-            while (d > 0 && hist[d] < left) left -= hist[d--];
-            s_digit = (uint32_t)d;
-            s_want = left;
+        // thread t holds kPer bins, counted from the top; the digit is the bin where the running count reaches want
+        int c[kPer], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sum += c[i] = hist[kBins - 1 - (tid * kPer + i)];
+        int incl = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+        }
+        if (tid == 0) { s_digit = kBins - 1; s_want = want; }      // want 0: nothing is kept
+        int total, before = warp_offsets<W>(__shfl_sync(0xffffffffu, incl, 31), buf, total) + incl - sum;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (before < want && before + c[i] >= want) {
+                s_digit = kBins - 1 - (tid * kPer + i);
+                s_want = want - before;
+            }
+            before += c[i];
         }
         __syncthreads();
-        prefix |= s_digit << shift;
-        mask |= 255u << shift;
+        prefix |= ((uint32_t)s_digit & digits) << shift;
+        mask |= digits << shift;
         want = s_want;
         __syncthreads();
     }
     // keys above `prefix` are kept, of those equal to it the first `want`. A
     // warp owns whole groups of 32 slots, in order.
-    const int groups = (n + 31) / 32, per = (groups + kSelWarps - 1) / kSelWarps;
+    const int groups = (n + 31) / 32, per = (groups + W - 1) / W;
     const int g0 = min(warp * per, groups), g1 = min(g0 + per, groups);
     int ties = 0;
     for (int g = g0; g < g1; ++g) {
@@ -127,7 +172,7 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictArgs a, boo
         ties += __popc(__ballot_sync(0xffffffffu, i < n && key_of(i) == prefix));
     }
     int total;
-    const int tie0 = warp_offsets(ties, buf, total);
+    const int tie0 = warp_offsets<W>(ties, buf, total);
     // pass 0 counts this warp's freed and moving slots, pass 1 writes them
     int hole_at = 0, from_at = 0, moves = 0;
     int2 *list = a.list + (size_t)pair * a.max_moves;
@@ -143,61 +188,66 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(EvictArgs a, boo
             const bool hole = i < a.budget && !keep, from = i >= a.budget && keep;   // budget < n
             const uint32_t hb = __ballot_sync(0xffffffffu, hole), fb = __ballot_sync(0xffffffffu, from);
             if (pass == 1) {
-                if (hole) list[holes + __popc(hb & below)].y = i;
-                if (from) list[froms + __popc(fb & below)].x = i;
+                const int h = holes + __popc(hb & below), f = froms + __popc(fb & below);
+                if (hole) (h < kSelMoves ? mine[h] : list[h]).y = i;
+                if (from) (f < kSelMoves ? mine[f] : list[f]).x = i;
             }
             holes += __popc(hb);
             froms += __popc(fb);
         }
         if (pass == 0) {
-            hole_at = warp_offsets(holes, buf, moves);
-            from_at = warp_offsets(froms, buf, moves);     // as many kept behind the budget as freed below it
+            hole_at = warp_offsets<W>(holes, buf, moves);
+            from_at = warp_offsets<W>(froms, buf, moves);  // as many kept behind the budget as freed below it
         }
     }
     if (tid == 0) a.count[pair] = moves;
+    __syncthreads();
+    const int here = min(moves, kSelMoves);
+    move_rows(a, pair, [&](int m) { return mine[m]; }, warp, here, W, lane);
+    for (int m = tid; m < here; m += THREADS) {
+        const size_t at = (size_t)pair * a.max_ctx;
+        a.weight_rw[at + mine[m].y] = w[mine[m].x];
+        a.slot_pos_rw[at + mine[m].y] = sp[mine[m].x];
+    }
 }
 
-constexpr int kMoveWarps = 8, kMovePer = 4;        // moves of a warp in flight
+constexpr int kMoveWarps = 8;
 constexpr int kMoveChunk = kMoveWarps * kMovePer;  // moves per block and step
 
 __global__ void __launch_bounds__(kMoveWarps * kWarp) kv_move_kernel(EvictArgs a, int chunks) {
     grid_dep_wait();
     grid_dep_launch_dependents();
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    for (int s = blockIdx.x * kMoveWarps * kWarp + threadIdx.x; s < a.n_pairs / a.Hkv; s += gridDim.x * kMoveWarps * kWarp)
+        if (a.len[s] > a.budget && a.len[s] <= a.max_ctx) a.len[s] = a.budget;
     const int64_t items = (int64_t)a.n_pairs * chunks;
     for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
         const int pair = (int)(it / chunks), chunk = (int)(it % chunks);
-        const int s = pair / a.Hkv, j = pair % a.Hkv;
-        const int n = a.count[pair];
-        if (chunk == 0 && j == 0 && threadIdx.x == 0 && a.len[s] > a.budget && a.len[s] <= a.max_ctx)
-            a.len[s] = a.budget;
-        const int m0 = chunk * kMoveChunk + warp * kMovePer;
+        const int n = a.count[pair], m0 = kSelMoves + chunk * kMoveChunk;
         if (m0 >= n) continue;
         const int2 *list = a.list + (size_t)pair * a.max_moves;
-        // lanes 0-15 carry the K row, 16-31 the V row, 16 bytes each
-        __half *base = (lane < 16 ? a.k : a.v) + ((size_t)s * a.max_ctx * a.Hkv + j) * kKvD + (lane & 15) * 8;
-        const size_t stride = (size_t)a.Hkv * kKvD;
-        int2 mv[kMovePer];
-        uint4 d[kMovePer];
-#pragma unroll
-        for (int i = 0; i < kMovePer; ++i)
-            if (m0 + i < n) mv[i] = list[m0 + i];
-#pragma unroll
-        for (int i = 0; i < kMovePer; ++i)
-            if (m0 + i < n) d[i] = *reinterpret_cast<const uint4 *>(base + (size_t)mv[i].x * stride);
-#pragma unroll
-        for (int i = 0; i < kMovePer; ++i)
-            if (m0 + i < n) *reinterpret_cast<uint4 *>(base + (size_t)mv[i].y * stride) = d[i];
-        if (lane < kMovePer && m0 + lane < n) {
-            const int2 m = list[m0 + lane];
+        const int end = min(n, m0 + kMoveChunk);
+        move_rows(a, pair, [&](int m) { return list[m]; }, m0 + warp, end, kMoveWarps, lane);
+        const int m = m0 + threadIdx.x;
+        if (m < end) {
             const size_t at = (size_t)pair * a.max_ctx;
-            a.weight_rw[at + m.y] = a.weight_rw[at + m.x];
-            a.slot_pos_rw[at + m.y] = a.slot_pos_rw[at + m.x];
+            a.weight_rw[at + list[m].y] = a.weight_rw[at + list[m].x];
+            a.slot_pos_rw[at + list[m].y] = a.slot_pos_rw[at + list[m].x];
         }
     }
 }
 
 size_t al256(size_t v) { return (v + 255) / 256 * 256; }
+
+template <int THREADS>
+int launch_select(const EvictArgs &a, bool cached, size_t smem, cudaStream_t s) {
+    if (smem > 32 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kv_select_kernel<THREADS>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kSelCacheMax * 4);
+        if (e != cudaSuccess) return (int)e;
+    }
+    return (int)launch_pdl(kv_select_kernel<THREADS>, dim3((unsigned)a.n_pairs), dim3(THREADS), smem, s, true, a, cached);
+}
 
 int moves_max(const li_kv_cache *C, int budget) {
     return budget < C->max_ctx - budget ? budget : C->max_ctx - budget;
@@ -238,16 +288,13 @@ int li_launch_kv_evict(const li_kv_cache *C, const int32_t *pos, int budget, int
     const cudaStream_t st = (cudaStream_t)stream;
     const bool cached = C->max_ctx <= kSelCacheMax;
     const size_t smem = cached ? (size_t)C->max_ctx * 4 : 0;
-    if (smem > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kv_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   kSelCacheMax * 4);
-        if (e != cudaSuccess) return (int)e;
-    }
-    int rc = (int)launch_pdl(kv_select_kernel, dim3((unsigned)pairs), dim3(kSelThreads), smem, st, true, a, cached);
+    int rc = C->max_ctx < kSelWide ? launch_select<512>(a, cached, smem, st) : launch_select<1024>(a, cached, smem, st);
     if (rc) return rc;
-    const int chunks = a.max_moves > 0 ? (a.max_moves + kMoveChunk - 1) / kMoveChunk : 1;
+    const int chunks = a.max_moves > kSelMoves ? (a.max_moves - kSelMoves + kMoveChunk - 1) / kMoveChunk : 0;
     const int64_t items = (int64_t)pairs * chunks, cap = (int64_t)num_sms() * 8;
-    return (int)launch_pdl(kv_move_kernel, dim3((unsigned)(items < cap ? items : cap)), dim3(kMoveWarps * kWarp), 0,
+    const int64_t lens = (C->n_seqs + kMoveWarps * kWarp - 1) / (kMoveWarps * kWarp);
+    const int64_t grid = items > lens ? items : lens;
+    return (int)launch_pdl(kv_move_kernel, dim3((unsigned)(grid < cap ? grid : cap)), dim3(kMoveWarps * kWarp), 0,
                            st, true, a, chunks);
 }
 

@@ -10,8 +10,10 @@
 // A thread's unit of work is two vectors of E values (16 bytes each where
 // alignment and sizes allow): the two halves of E pairs in the half layout,
 // 2E neighbouring values in the interleaved one, so that the layouts differ
-// only in which values of the unit form a pair. The first units' loads are
-// issued before the angles are computed, which hides the one behind the other.
+// only in which values of the unit form a pair. A thread keeps its place in
+// the head and walks over heads and tokens (no division per unit, the cos and
+// sin of a token in registers); the first units' loads are issued before the
+// angles are computed, which hides the one behind the other.
 #include "li_kv.cuh"
 
 #include <math.h>
@@ -57,7 +59,7 @@ int rope_args(const li_rope *R, RopeArgs *a) {
 
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 256;      // at most
 constexpr int kRopeBatch = 4;          // units of a thread in flight
 
 // One launch over n_tokens tokens and `heads` head slots. Plain rotation: one
@@ -70,6 +72,7 @@ struct RopeJob {
     const int32_t *pos;
     int n_tokens, heads, D;
     int tb, hb, n_hblk;                // tokens and head slots per block, head blocks
+    int hp, np;                        // heads a block takes at once, rounds of them per token
     int n_rot, units;                  // rotated units and all units per head
     float sin_sign;                    // -1: the transpose
     // append
@@ -121,69 +124,51 @@ template <typename T, int E, bool HALF, bool APPEND>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeJob j) {
     extern __shared__ __align__(16) uint8_t rope_smem[];
     const int half = j.r.rope_dim / 2;
-    int64_t *row = reinterpret_cast<int64_t *>(rope_smem);                            // [tb] cache row or -1
-    float2 *cs = reinterpret_cast<float2 *>(rope_smem + (APPEND ? 8 * j.tb : 0));     // [tb][half]
+    float2 *cs = reinterpret_cast<float2 *>(rope_smem);                               // [tb][half]
+    int64_t *row = reinterpret_cast<int64_t *>(rope_smem + (size_t)8 * j.tb * half);  // [tb] cache row or -1
     grid_dep_wait();
     grid_dep_launch_dependents();
-    const int tblk = blockIdx.x / j.n_hblk, hblk = blockIdx.x % j.n_hblk;
+    const int tblk = blockIdx.x / j.n_hblk, hblk = blockIdx.x - tblk * j.n_hblk;
     const int t0 = tblk * j.tb, nt = min(j.tb, j.n_tokens - t0);
     const int h0 = hblk * j.hb, nh = min(j.hb, j.heads - h0);
-    const int per_tok = nh * j.units, total = nt * per_tok;
-
-    struct Unit {
-        int tok, u, kind;              // kind 0: q or plain, 1: k, 2: v
-        int oa, ob;
-        const T *src;
-        int64_t dst;                   // element offset in the destination, -1: not stored
+    // this thread's place: unit u of head hd (of hp heads), the same in every round
+    const int hd = threadIdx.x / j.units, u = threadIdx.x - hd * j.units;
+    const bool rot = u < j.n_rot, worker = hd < j.hp;
+    const int oa = rot ? (HALF ? u * E : u * 2 * E) : j.r.rope_dim + (u - j.n_rot) * 2 * E;
+    const int ob = rot && HALF ? half + u * E : oa + E;
+    const bool two = ob < j.D;
+    // a walk over (token, round): the unit at (t, p) is head h0 + hd + p hp of token t0 + t
+    struct Walk { int t, p; };
+    auto step = [&](Walk &w) {
+        if (++w.p == j.np) { w.p = 0; ++w.t; }
     };
-    auto locate = [&](int idx) {
-        Unit w;
-        w.tok = idx / per_tok;
-        const int in = idx - w.tok * per_tok, hd = in / j.units;
-        w.u = in - hd * j.units;
-        const int h = h0 + hd, t = t0 + w.tok;
-        if (w.u < j.n_rot) {
-            w.oa = HALF ? w.u * E : w.u * 2 * E;
-            w.ob = HALF ? half + w.u * E : w.oa + E;
-        } else {
-            w.oa = j.r.rope_dim + (w.u - j.n_rot) * 2 * E;
-            w.ob = w.oa + E;
-        }
-        if (!APPEND || h < j.Hq) {
-            w.kind = 0;
-            w.src = static_cast<const T *>(j.x) + t * j.x_ts + h * j.x_hs;
-            w.dst = t * j.d_ts + h * j.d_hs;
-        } else if (h < j.Hq + j.Hkv) {
-            w.kind = 1;
-            w.src = static_cast<const T *>(j.k) + t * j.k_ts + (int64_t)(h - j.Hq) * j.D;
-            w.dst = h - j.Hq;
-        } else {
-            w.kind = 2;
-            w.src = static_cast<const T *>(j.v) + t * j.v_ts + (int64_t)(h - j.Hq - j.Hkv) * j.D;
-            w.dst = h - j.Hq - j.Hkv;
-        }
-        return w;
-    };
+    auto valid = [&](const Walk &w) { return worker && w.t < nt && hd + w.p * j.hp < nh; };
 
-    for (int base = threadIdx.x; base < total || base == (int)threadIdx.x; base += kRopeBatch * kRopeThreads) {
+    Walk ld = {0, 0}, wk = {0, 0};
+    int have = -1;                                  // token whose cos and sin are in c
+    float2 c[E];
+    for (bool first = true; wk.t < nt; first = false) {
         Pack<T, E> a[kRopeBatch], b[kRopeBatch];
 #pragma unroll
-        for (int i = 0; i < kRopeBatch; ++i) {
-            const int idx = base + i * kRopeThreads;
-            if (idx < total) {
-                const Unit w = locate(idx);
-                a[i] = load_pack<T, E>(w.src + w.oa);
-                if (w.ob < j.D) b[i] = load_pack<T, E>(w.src + w.ob);
-            }
+        for (int i = 0; i < kRopeBatch; ++i, step(ld)) {
+            if (!valid(ld)) continue;
+            const int h = h0 + hd + ld.p * j.hp;
+            const int64_t t = t0 + ld.t;
+            const T *src;
+            if (!APPEND || h < j.Hq) src = static_cast<const T *>(j.x) + t * j.x_ts + h * j.x_hs;
+            else if (h < j.Hq + j.Hkv) src = static_cast<const T *>(j.k) + t * j.k_ts + (int64_t)(h - j.Hq) * j.D;
+            else src = static_cast<const T *>(j.v) + t * j.v_ts + (int64_t)(h - j.Hq - j.Hkv) * j.D;
+            a[i] = load_pack<T, E>(src + oa);
+            if (two) b[i] = load_pack<T, E>(src + ob);
         }
-        if (base == (int)threadIdx.x) {            // the first round of every thread: the block's angles
-            for (int i = threadIdx.x; i < nt * half; i += kRopeThreads) {
+        if (first) {                                // the block's angles, behind the first loads
+            for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
                 const int tok = i / half;
-                float2 c = rope_cos_sin(j.r, j.pos[t0 + tok], i - tok * half);
-                c.y *= j.sin_sign;
-                cs[i] = c;
+                float2 x = rope_cos_sin(j.r, j.pos[t0 + tok], i - tok * half);
+                x.y *= j.sin_sign;
+                cs[i] = x;
             }
-            if (APPEND && threadIdx.x < nt) {
+            if (APPEND && (int)threadIdx.x < nt) {
                 const int t = t0 + threadIdx.x, s = j.seq ? j.seq[t] : t;
                 int64_t r = -1;
                 if (s >= 0 && s < j.n_seqs) {
@@ -196,53 +181,46 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
             __syncthreads();
         }
 #pragma unroll
-        for (int i = 0; i < kRopeBatch; ++i) {
-            const int idx = base + i * kRopeThreads;
-            if (idx >= total) break;
-            const Unit w = locate(idx);
+        for (int i = 0; i < kRopeBatch; ++i, step(wk)) {
+            if (!valid(wk)) continue;
+            const int h = h0 + hd + wk.p * j.hp;
+            const int64_t t = t0 + wk.t;
             float x[2][E];
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 x[0][e] = to_f(a[i].v[e]);
-                x[1][e] = w.ob < j.D ? to_f(b[i].v[e]) : 0.f;
+                x[1][e] = two ? to_f(b[i].v[e]) : 0.f;
             }
-            if (w.u < j.n_rot && w.kind < 2) {
-                const float2 *c = cs + w.tok * half + w.u * E;
-                if (HALF) {
+            if (rot && (!APPEND || h < j.Hq + j.Hkv)) {
+                if (wk.t != have) {
+                    have = wk.t;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const float2 t = c[e];
-                        const float p = x[0][e], q = x[1][e];
-                        x[0][e] = p * t.x - q * t.y;
-                        x[1][e] = q * t.x + p * t.y;
-                    }
-                } else {
+                    for (int e = 0; e < E; ++e) c[e] = cs[wk.t * half + u * E + e];
+                }
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const float2 t = c[e];
-                        float &lo = x[(2 * e) / E][(2 * e) % E], &hi = x[(2 * e + 1) / E][(2 * e + 1) % E];
-                        const float p = lo, q = hi;
-                        lo = p * t.x - q * t.y;
-                        hi = q * t.x + p * t.y;
-                    }
+                for (int e = 0; e < E; ++e) {
+                    // pair e of the unit: (a_e, b_e), or values 2e and 2e + 1 of the 2E neighbours
+                    float &lo = HALF ? x[0][e] : x[(2 * e) / E][(2 * e) % E];
+                    float &hi = HALF ? x[1][e] : x[(2 * e + 1) / E][(2 * e + 1) % E];
+                    const float p = lo, q = hi;
+                    lo = p * c[e].x - q * c[e].y;
+                    hi = q * c[e].x + p * c[e].y;
                 }
             }
-            if (!APPEND || w.kind == 0) {
-                T *o = static_cast<T *>(j.dst) + w.dst;
-                store_pack<T, E>(o + w.oa, x[0]);
-                if (w.ob < j.D) store_pack<T, E>(o + w.ob, x[1]);
-            } else {
-                const int64_t r = row[w.tok];
-                if (r >= 0) {
-                    __half *o = (w.kind == 1 ? j.k_cache : j.v_cache) + (r * j.Hkv + w.dst) * j.D;
-                    store_pack<__half, E>(o + w.oa, x[0]);
-                    if (w.ob < j.D) store_pack<__half, E>(o + w.ob, x[1]);
-                }
+            if (!APPEND || h < j.Hq) {
+                T *o = static_cast<T *>(j.dst) + t * j.d_ts + h * j.d_hs;
+                store_pack<T, E>(o + oa, x[0]);
+                if (two) store_pack<T, E>(o + ob, x[1]);
+            } else if (const int64_t r = row[wk.t]; r >= 0) {
+                const bool is_k = h < j.Hq + j.Hkv;
+                __half *o = (is_k ? j.k_cache : j.v_cache) + (r * j.Hkv + h - j.Hq - (is_k ? 0 : j.Hkv)) * j.D;
+                store_pack<__half, E>(o + oa, x[0]);
+                if (two) store_pack<__half, E>(o + ob, x[1]);
             }
         }
     }
     if (APPEND && hblk == 0 && (j.weight || j.slot_pos)) {
-        for (int i = threadIdx.x; i < nt * j.Hkv; i += kRopeThreads) {
+        for (int i = threadIdx.x; i < nt * j.Hkv; i += blockDim.x) {
             const int tok = i / j.Hkv, hd = i - tok * j.Hkv;
             const int64_t r = row[tok];
             if (r < 0) continue;
@@ -254,49 +232,53 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
 }
 
 template <typename T, int E, bool APPEND>
-int rope_go(const RopeJob &j, unsigned grid, size_t smem, cudaStream_t s) {
+int rope_go(const RopeJob &j, unsigned grid, unsigned threads, size_t smem, cudaStream_t s) {
     if (j.r.layout == LI_ROPE_HALF)
-        return (int)launch_pdl(rope_kernel<T, E, true, APPEND>, dim3(grid), dim3(kRopeThreads), smem, s, true, j);
-    return (int)launch_pdl(rope_kernel<T, E, false, APPEND>, dim3(grid), dim3(kRopeThreads), smem, s, true, j);
+        return (int)launch_pdl(rope_kernel<T, E, true, APPEND>, dim3(grid), dim3(threads), smem, s, true, j);
+    return (int)launch_pdl(rope_kernel<T, E, false, APPEND>, dim3(grid), dim3(threads), smem, s, true, j);
 }
 
-// Splits the work into blocks of about kRopeBatch units a thread (whole
-// tokens; a token with more than twice that, or a call of few tokens, is split
-// over its heads too, so that small calls still spread over the SMs) and
-// launches with the widest vectors that sizes and addresses allow.
+// Launches with the widest vectors that sizes and addresses allow, in blocks
+// of whole tokens with about kRopeBatch units a thread; a call of few tokens
+// is split over the heads too, so that it still spreads over the SMs.
 template <typename T, bool APPEND>
 int rope_launch(RopeJob &j, int e_max, cudaStream_t s) {
     int E = e_max;
     while (E > 1 && (j.r.rope_dim % (2 * E) || (j.D - j.r.rope_dim) % E)) E >>= 1;
     j.n_rot = j.r.rope_dim / (2 * E);
-    j.units = j.n_rot + (j.D - j.r.rope_dim + 2 * E - 1) / (2 * E);
+    j.units = j.n_rot + (j.D - j.r.rope_dim + 2 * E - 1) / (2 * E);      // at most 256: head_dim <= 512
+    const int64_t per_tok = (int64_t)j.heads * j.units, all = per_tok * j.n_tokens;
     const int want = kRopeBatch * kRopeThreads;
-    const int64_t per_tok = (int64_t)j.heads * j.units;
+    // units per block: all SMs busy first, then kRopeBatch a thread
+    int64_t share = (all + num_sms() - 1) / num_sms();
+    share = share < kRopeThreads ? kRopeThreads : share < want ? share : want;
     j.tb = 1;
     j.hb = j.heads;
-    if (per_tok * j.n_tokens < (int64_t)want * num_sms()) {
-        // fewer units than the SMs' threads take at once: one unit a thread, if it comes to that
-        const int64_t share = (per_tok * j.n_tokens + num_sms() - 1) / num_sms();
-        const int64_t heads = (share < kRopeThreads ? kRopeThreads : share) / j.units;
-        j.hb = (int)(heads < 1 ? 1 : heads < j.heads ? heads : j.heads);
-    } else if (per_tok > 2 * want) {
-        j.hb = want / j.units < 1 ? 1 : want / j.units;
-    } else if (per_tok < want) {
-        j.tb = (int)(want / per_tok);
+    if (per_tok > share) {
+        const int64_t blocks = (per_tok + share - 1) / share;           // of about equally many heads
+        j.hb = (int)((j.heads + blocks - 1) / blocks);
+    } else {
+        j.tb = (int)(share / per_tok);
+        const int tb_max = 16384 / (8 + 4 * j.r.rope_dim);              // 16 KB of angles
+        if (j.tb > tb_max) j.tb = tb_max;
+        if (j.tb > j.n_tokens) j.tb = j.n_tokens;
     }
-    const int tb_max = 16384 / (8 + 4 * j.r.rope_dim);      // 16 KB of angles
-    if (j.tb > tb_max) j.tb = tb_max;
-    if (j.tb > kRopeThreads) j.tb = kRopeThreads;
     j.n_hblk = (j.heads + j.hb - 1) / j.hb;
+    // as many heads at once as 256 threads hold, in rounds of about equally many
+    const int fit = kRopeThreads / j.units;
+    j.np = (j.hb + fit - 1) / fit;
+    j.hp = (j.hb + j.np - 1) / j.np;
+    int threads = (j.hp * j.units + 31) / 32 * 32;
+    if (threads < j.tb) threads = (j.tb + 31) / 32 * 32;                // a token each for the cache rows
     const int64_t grid = (int64_t)((j.n_tokens + j.tb - 1) / j.tb) * j.n_hblk;
     if (grid > 0x7fffffff) return LI_ERR_BAD_SHAPE;
-    const size_t smem = (size_t)j.tb * ((APPEND ? 8 : 0) + 4 * j.r.rope_dim);
+    const size_t smem = (size_t)j.tb * (4 * j.r.rope_dim + (APPEND ? 8 : 0));
     if constexpr (sizeof(T) == 2)
-        if (E == 8) return rope_go<T, 8, APPEND>(j, (unsigned)grid, smem, s);
+        if (E == 8) return rope_go<T, 8, APPEND>(j, (unsigned)grid, (unsigned)threads, smem, s);
     switch (E) {
-    case 4: return rope_go<T, 4, APPEND>(j, (unsigned)grid, smem, s);
-    case 2: return rope_go<T, 2, APPEND>(j, (unsigned)grid, smem, s);
-    default: return rope_go<T, 1, APPEND>(j, (unsigned)grid, smem, s);
+    case 4: return rope_go<T, 4, APPEND>(j, (unsigned)grid, (unsigned)threads, smem, s);
+    case 2: return rope_go<T, 2, APPEND>(j, (unsigned)grid, (unsigned)threads, smem, s);
+    default: return rope_go<T, 1, APPEND>(j, (unsigned)grid, (unsigned)threads, smem, s);
     }
 }
 
