@@ -11,8 +11,8 @@
 // alignment and sizes allow): the two halves of E pairs in the half layout,
 // 2E neighbouring values in the interleaved one, so that the layouts differ
 // only in which values of the unit form a pair. A thread keeps its place in
-// the head and walks over heads and tokens (no division per unit, the cos and
-// sin of a token in registers); the first units' loads are issued before the
+// the head and walks over heads and tokens (no division per unit); the first
+// units' loads are issued before the
 // angles are computed, which hides the one behind the other.
 #include "li_kv.cuh"
 
@@ -60,7 +60,11 @@ int rope_args(const li_rope *R, RopeArgs *a) {
 namespace {
 
 constexpr int kRopeThreads = 256;      // at most
-constexpr int kRopeBatch = 4;          // units of a thread in flight
+// Units of a thread in flight, and blocks per SM that the registers are held
+// down to: more of the one costs the other. Two and four took 24.9 us for 4096
+// tokens x 48 heads x 128 bf16 (of 15.6 at the copy rate), four units without
+// a bound 36 us, three 33 us, two at five blocks 30 us.
+constexpr int kRopeBatch = 2, kRopeBlocks = 4;
 
 // One launch over n_tokens tokens and `heads` head slots. Plain rotation: one
 // source. Append: head slots are q heads, then k heads, then v heads.
@@ -121,7 +125,7 @@ __device__ __forceinline__ void store_pack(O *p, const float (&f)[E]) {
 }
 
 template <typename T, int E, bool HALF, bool APPEND>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeJob j) {
+__global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_kernel(const __grid_constant__ RopeJob j) {
     extern __shared__ __align__(16) uint8_t rope_smem[];
     const int half = j.r.rope_dim / 2;
     float2 *cs = reinterpret_cast<float2 *>(rope_smem);                               // [tb][half]
@@ -145,8 +149,6 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
     auto valid = [&](const Walk &w) { return worker && w.t < nt && hd + w.p * j.hp < nh; };
 
     Walk ld = {0, 0}, wk = {0, 0};
-    int have = -1;                                  // token whose cos and sin are in c
-    float2 c[E];
     for (bool first = true; wk.t < nt; first = false) {
         Pack<T, E> a[kRopeBatch], b[kRopeBatch];
 #pragma unroll
@@ -192,19 +194,16 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
                 x[1][e] = two ? to_f(b[i].v[e]) : 0.f;
             }
             if (rot && (!APPEND || h < j.Hq + j.Hkv)) {
-                if (wk.t != have) {
-                    have = wk.t;
-#pragma unroll
-                    for (int e = 0; e < E; ++e) c[e] = cs[wk.t * half + u * E + e];
-                }
+                const float2 *cp = cs + wk.t * half + u * E;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     // pair e of the unit: (a_e, b_e), or values 2e and 2e + 1 of the 2E neighbours
                     float &lo = HALF ? x[0][e] : x[(2 * e) / E][(2 * e) % E];
                     float &hi = HALF ? x[1][e] : x[(2 * e + 1) / E][(2 * e + 1) % E];
                     const float p = lo, q = hi;
-                    lo = p * c[e].x - q * c[e].y;
-                    hi = q * c[e].x + p * c[e].y;
+                    const float2 c = cp[e];
+                    lo = p * c.x - q * c.y;
+                    hi = q * c.x + p * c.y;
                 }
             }
             if (!APPEND || h < j.Hq) {
@@ -239,7 +238,7 @@ int rope_go(const RopeJob &j, unsigned grid, unsigned threads, size_t smem, cuda
 }
 
 // Launches with the widest vectors that sizes and addresses allow, in blocks
-// of whole tokens with about kRopeBatch units a thread; a call of few tokens
+// of whole tokens with about 2 kRopeBatch units a thread; a call of few tokens
 // is split over the heads too, so that it still spreads over the SMs.
 template <typename T, bool APPEND>
 int rope_launch(RopeJob &j, int e_max, cudaStream_t s) {
@@ -248,8 +247,8 @@ int rope_launch(RopeJob &j, int e_max, cudaStream_t s) {
     j.n_rot = j.r.rope_dim / (2 * E);
     j.units = j.n_rot + (j.D - j.r.rope_dim + 2 * E - 1) / (2 * E);      // at most 256: head_dim <= 512
     const int64_t per_tok = (int64_t)j.heads * j.units, all = per_tok * j.n_tokens;
-    const int want = kRopeBatch * kRopeThreads;
-    // units per block: all SMs busy first, then kRopeBatch a thread
+    const int want = 2 * kRopeBatch * kRopeThreads;                     // two rounds a thread
+    // units per block: all SMs busy first, then two rounds a thread
     int64_t share = (all + num_sms() - 1) / num_sms();
     share = share < kRopeThreads ? kRopeThreads : share < want ? share : want;
     j.tb = 1;

@@ -28,7 +28,8 @@ __all__ = [
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # the raw handle of torch.cuda.current_stream(), without building the Stream object around it
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _p(t: torch.Tensor | None) -> int | None:
@@ -328,27 +329,29 @@ _DTYPES = {torch.float32: LI_DTYPE_F32, torch.float16: LI_DTYPE_F16, torch.bfloa
 _ROPE_LAYOUTS = {"interleaved": LI_ROPE_INTERLEAVED, "half": LI_ROPE_HALF}
 
 
-def _dev(device: torch.device, *tensors, dtype=None) -> None:
-    """The tensors lie on `device`, and it is the current one (the library
-    launches on the current device's stream)."""
-    if device.type != "cuda":
-        raise ValueError("LeanInfer kernels take CUDA tensors")
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"tensors on {device}, but cuda:{torch.cuda.current_device()} is the current device")
+def _on(index: int, *tensors) -> None:
+    """The tensors lie on cuda:index, and it is the current device (the
+    library launches on the current device's stream)."""
     for t in tensors:
-        if t is not None:
-            if t.device != device:
-                raise ValueError(f"tensors on {t.device} and {device}")
-            if dtype is not None and t.dtype != dtype:
-                raise ValueError(f"expected {dtype}, got {t.dtype}")
+        if t is not None and t.get_device() != index:
+            raise ValueError("LeanInfer kernels take CUDA tensors of one device")
+    if index < 0:
+        raise ValueError("LeanInfer kernels take CUDA tensors")
+    if index != torch.cuda.current_device():
+        raise ValueError(f"tensors on cuda:{index}, but cuda:{torch.cuda.current_device()} is the current device")
 
 
-def _heads(t: torch.Tensor, n: int, heads: int | None, dim: int, what: str) -> None:
-    """[n, heads, dim] with each token's heads contiguous; any token stride."""
-    if t.dim() != 3 or t.shape[0] != n or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{what}: expected [{n}, {heads or 'heads'}, {dim}], got {tuple(t.shape)}")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim):
+def _heads(t: torch.Tensor, n: int, heads: int | None, dim: int, dtype, what: str) -> int:
+    """Checks [n, heads, dim] with each token's heads contiguous and any token
+    stride; returns that stride."""
+    shape, st = t.shape, t.stride()
+    if len(shape) != 3 or shape[0] != n or shape[2] != dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what}: expected [{n}, {heads or 'heads'}, {dim}], got {tuple(shape)}")
+    if st[2] != 1 or (st[1] != dim and shape[1] > 1):
         raise ValueError(f"{what}: the heads of a token must be contiguous")
+    if t.dtype != dtype:
+        raise ValueError(f"{what}: expected {dtype}, got {t.dtype}")
+    return st[0]
 
 
 def _index(t: torch.Tensor | None, n: int, what: str) -> int | None:
@@ -394,11 +397,12 @@ def rope(rope: Rope, x: torch.Tensor, pos: torch.Tensor, out: torch.Tensor | Non
         raise ValueError("out: expected the shape of x with contiguous heads")
     if x.dtype not in _DTYPES:
         raise ValueError(f"x: {x.dtype} is not fp32, fp16 or bf16")
-    _dev(x.device, out, dtype=x.dtype)
-    _dev(x.device, pos, rope.keep)
+    if out.dtype != x.dtype:
+        raise ValueError(f"out: expected {x.dtype}, got {out.dtype}")
+    _on(x.get_device(), out, pos, rope.keep)
+    xs, os = x.stride(), out.stride()
     check(_lib.load().li_launch_rope(rope.ref, _DTYPES[x.dtype], x.data_ptr(), out.data_ptr(), _index(pos, n, "pos"),
-                                     n, heads, x.stride(0), x.stride(1), out.stride(0), out.stride(1), int(transpose),
-                                     _stream()), "li_launch_rope")
+                                     n, heads, xs[0], xs[1], os[0], os[1], transpose, _stream()), "li_launch_rope")
     return out
 
 
@@ -412,7 +416,7 @@ class KVCache:
 
     def __init__(self, k, v, len, *, k_prefix=None, v_prefix=None, weight=None, slot_pos=None):
         n, ctx, heads, dim = k.shape
-        self.device = k.device
+        self.device, self.index = k.device, k.get_device()
         if v.shape != k.shape:
             raise ValueError("k and v differ in shape")
         if (k_prefix is None) != (v_prefix is None):
@@ -448,44 +452,41 @@ class KVCache:
         (seq[t], slot[t]); without seq, token t is sequence t's, without slot
         it goes to slot len - 1. Returns q rotated (q_out, which may be q), or
         None without q."""
-        n = k.shape[0]
-        if k.dtype not in _DTYPES:
-            raise ValueError(f"k: {k.dtype} is not fp32, fp16 or bf16")
-        _heads(k, n, self.n_kv_heads, self.head_dim, "k")
-        _heads(v, n, self.n_kv_heads, self.head_dim, "v")
-        _dev(self.device, k, v, q, q_out, dtype=k.dtype)
-        _dev(self.device, pos, seq, slot, rope.keep if rope is not None else None)
+        n, dt, dim = k.shape[0], k.dtype, self.head_dim
+        if dt not in _DTYPES:
+            raise ValueError(f"k: {dt} is not fp32, fp16 or bf16")
+        ks, vs = _heads(k, n, self.n_kv_heads, dim, dt, "k"), _heads(v, n, self.n_kv_heads, dim, dt, "v")
+        _on(self.index, k, v, q, q_out, pos, seq, slot, rope.keep if rope is not None else None)
         qp = op = None
         qs = os = hq = 0
         if q is not None:
             hq = q.shape[1]
-            _heads(q, n, hq, self.head_dim, "q")
+            qs = _heads(q, n, hq, dim, dt, "q")
             if q_out is None:
-                q_out = torch.empty(n, hq, self.head_dim, device=self.device, dtype=q.dtype)
-            else:
-                _heads(q_out, n, hq, self.head_dim, "q_out")
-            qp, op, qs, os = q.data_ptr(), q_out.data_ptr(), q.stride(0), q_out.stride(0)
+                q_out = torch.empty(n, hq, dim, device=self.device, dtype=dt)
+            os = _heads(q_out, n, hq, dim, dt, "q_out")
+            qp, op = q.data_ptr(), q_out.data_ptr()
         check(_lib.load().li_launch_kv_append(
-            self.ref, rope.ref if rope is not None else None, _DTYPES[k.dtype], qp, qs, op, os, hq, k.data_ptr(),
-            k.stride(0), v.data_ptr(), v.stride(0), _index(pos, n, "pos"), _index(seq, n, "seq"),
-            _index(slot, n, "slot"), n, _stream()), "li_launch_kv_append")
+            self.ref, rope.ref if rope is not None else None, _DTYPES[dt], qp, qs, op, os, hq, k.data_ptr(), ks,
+            v.data_ptr(), vs, _index(pos, n, "pos"), _index(seq, n, "seq"), _index(slot, n, "slot"), n, _stream()),
+            "li_launch_kv_append")
         return q_out if q is not None else None
 
     def decode(self, q, *, scale: float | None = None, decay: float = 1.0, out=None, workspace=None):
         """Attention of q [n_seqs, n_q_heads, 128] (fp32) over the prefix and
         each sequence's first len slots; returns [n_seqs, n_q_heads, 128]. With
         weight in the cache, weight = decay * weight + this step's."""
-        _heads(q, self.n_seqs, None, self.head_dim, "q")
+        qs = _heads(q, self.n_seqs, None, self.head_dim, torch.float32, "q")
         hq = q.shape[1]
         if out is None:
             out = torch.empty(self.n_seqs, hq, self.head_dim, device=self.device, dtype=torch.float32)
-        elif out.shape != q.shape or not out.is_contiguous():
-            raise ValueError("out: expected a contiguous tensor of q's shape")
-        _dev(self.device, q, out, dtype=torch.float32)
+        elif out.shape != q.shape or not out.is_contiguous() or out.dtype != torch.float32:
+            raise ValueError("out: expected a contiguous fp32 tensor of q's shape")
+        _on(self.index, q, out, workspace)
         lib = _lib.load()
         ws = workspace if workspace is not None else self._workspace(
             hq, lambda: int(lib.li_attn_kv_workspace_size(self.ref, hq)))
-        check(lib.li_launch_attn_kv_decode(self.ref, q.data_ptr(), q.stride(0), hq,
+        check(lib.li_launch_attn_kv_decode(self.ref, q.data_ptr(), qs, hq,
                                            self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), decay,
                                            ws.data_ptr(), ws.numel(), _stream()), "li_launch_attn_kv_decode")
         return out
@@ -494,7 +495,7 @@ class KVCache:
         """Shrinks every longer sequence to `budget` slots by weight (see
         li_launch_kv_evict); pos int32 [n_seqs], the newest token's position;
         n_sink counts own tokens, after the prefix."""
-        _dev(self.device, pos)
+        _on(self.index, pos, workspace)
         lib = _lib.load()
         ws = workspace if workspace is not None else self._workspace(
             ("evict", budget), lambda: int(lib.li_kv_evict_workspace_size(self.ref, budget)))
