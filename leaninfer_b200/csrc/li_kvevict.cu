@@ -11,7 +11,7 @@
 //
 //   kv_select   block per (sequence, kv head): the budget-th largest key by a
 //               radix search over digits of 11, 11 and 10 bits, the two
-//               ascending lists by warp ballots and a block scan, and the first
+//               ascending lists from a bit mask of the kept slots, and the first
 //               kSelMoves moves themselves: 512 bytes (K and V row) each, plus
 //               weight and position, eight a warp in flight. That is all there
 //               is where a cache overshoots its budget by a little, as it does
@@ -26,7 +26,7 @@ namespace li {
 namespace {
 
 constexpr int kSelCacheMax = 48 * 1024;     // keys held in shared memory up to this many slots
-constexpr int kSelWide = 8192;              // from this many slots on, blocks of 1024 threads
+constexpr int kSelWide = 8192;              // from this many slots on, blocks of 1024 threads, below 512
 constexpr int kSelMoves = 256;              // moves that kv_select makes itself
 constexpr int kBins = 2048;                 // of a digit
 constexpr int kMovePer = 8;                 // moves of a warp in flight
@@ -39,6 +39,8 @@ struct EvictArgs {
     int64_t first_free;                // positions below are protected: the prefix's and the sinks'
     int32_t *count;                    // [n_seqs * Hkv] moves
     int2 *list;                        // [n_seqs * Hkv][max_moves] (from, to)
+    uint32_t *masks;                   // [n_seqs * Hkv][mask_words]: kept slots, where shared memory is short
+    int mask_words;                    // ceil(max_ctx / 32)
     __half *k, *v;
     float *weight_rw;
     int32_t *slot_pos_rw;
@@ -58,15 +60,15 @@ __device__ __forceinline__ int warp_offsets(int v, int *buf, int &total) {
     __syncthreads();
     if (lane == 0) buf[warp] = v;
     __syncthreads();
-    int off = 0, sum = 0;
+    int incl = lane < W ? buf[lane] : 0;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-        const int x = buf[w];
-        if (w < warp) off += x;
-        sum += x;
+    for (int o = 1; o < W; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += x;
     }
-    total = sum;
-    return off;
+    total = __shfl_sync(0xffffffffu, incl, W - 1);
+    const int before = __shfl_sync(0xffffffffu, incl, warp ? warp - 1 : 0);
+    return warp ? before : 0;
 }
 
 // Rows m, m + stride, ... of a pair's moves: lanes 0-15 carry the K row, 16-31
@@ -88,18 +90,18 @@ __device__ __forceinline__ void move_rows(const EvictArgs &a, int pair, List mov
 }
 
 template <int THREADS>
-__global__ void __launch_bounds__(THREADS) kv_select_kernel(EvictArgs a, bool cached) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv_select_kernel(EvictArgs a, bool cached) {
     constexpr int W = THREADS / kWarp, kPer = kBins / THREADS;
-    extern __shared__ uint32_t keys[];             // [max_ctx] when cached
+    extern __shared__ uint32_t keys[];             // cached: [max_ctx] keys, [mask_words] kept slots
     __shared__ int hist[kBins];
     __shared__ int buf[W];
-    __shared__ int s_digit, s_want;
+    __shared__ int s_digit, s_want, s_all;
     __shared__ int2 mine[kSelMoves];
     grid_dep_wait();
     grid_dep_launch_dependents();
     const int pair = blockIdx.x, s = pair / a.Hkv;
     const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
-    const int n = a.len[s];
+    const int n = a.len[s], newest = a.pos[s];
     if (n < 0 || n > a.max_ctx) {
         if (tid == 0) {
             atomicExch(&g_device_error, LI_ERR_BAD_ARG);
@@ -113,14 +115,11 @@ __global__ void __launch_bounds__(THREADS) kv_select_kernel(EvictArgs a, bool ca
     }
     const float *w = a.weight + (size_t)pair * a.max_ctx;
     const int32_t *sp = a.slot_pos + (size_t)pair * a.max_ctx;
-    const int64_t newest_free = (int64_t)a.pos[s] - a.n_recent;
+    const int64_t newest_free = (int64_t)newest - a.n_recent;
     auto key_of = [&](int i) -> uint32_t {
         return cached ? keys[i] : evict_key(w[i], sp[i], a.first_free, newest_free);
     };
-    if (cached) {
-#pragma unroll 4
-        for (int i = tid; i < n; i += THREADS) keys[i] = evict_key(w[i], sp[i], a.first_free, newest_free);
-    }
+    uint32_t *masks = cached ? keys + a.max_ctx : a.masks + (size_t)pair * a.mask_words;
     // the budget-th largest key, digit by digit from the top: `prefix` holds
     // the digits found, `want` the rank left among the keys that share them
     uint32_t prefix = 0, mask = 0;
@@ -131,9 +130,18 @@ __global__ void __launch_bounds__(THREADS) kv_select_kernel(EvictArgs a, bool ca
         const uint32_t digits = pass == 2 ? 1023u : 2047u;
         for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += THREADS) {
-            const uint32_t k = key_of(i);
-            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digits], 1);
+        if (pass == 0) {
+#pragma unroll 8
+            for (int i = tid; i < n; i += THREADS) {
+                const uint32_t k = evict_key(w[i], sp[i], a.first_free, newest_free);
+                if (cached) keys[i] = k;
+                atomicAdd(&hist[k >> shift], 1);
+            }
+        } else {
+            for (int i = tid; i < n; i += THREADS) {
+                const uint32_t k = key_of(i);
+                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digits], 1);
+            }
         }
         __syncthreads();
         // thread t holds kPer bins, counted from the top; the digit is the bin where the running count reaches want
@@ -146,13 +154,14 @@ __global__ void __launch_bounds__(THREADS) kv_select_kernel(EvictArgs a, bool ca
             const int x = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += x;
         }
-        if (tid == 0) { s_digit = kBins - 1; s_want = want; }      // want 0: nothing is kept
+        if (tid == 0) { s_digit = kBins - 1; s_want = s_all = want; }      // want 0: nothing is kept
         int total, before = warp_offsets<W>(__shfl_sync(0xffffffffu, incl, 31), buf, total) + incl - sum;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             if (before < want && before + c[i] >= want) {
                 s_digit = kBins - 1 - (tid * kPer + i);
                 s_want = want - before;
+                s_all = c[i];
             }
             before += c[i];
         }
@@ -162,53 +171,76 @@ __global__ void __launch_bounds__(THREADS) kv_select_kernel(EvictArgs a, bool ca
         want = s_want;
         __syncthreads();
     }
-    // keys above `prefix` are kept, of those equal to it the first `want`. A
-    // warp owns whole groups of 32 slots, in order.
+    // keys above `prefix` are kept, of those equal to it the first `want` (all
+    // of them, unless weights are tied at the border): a bit per slot. A warp
+    // owns whole groups of 32 slots, in order.
     const int groups = (n + 31) / 32, per = (groups + W - 1) / W;
     const int g0 = min(warp * per, groups), g1 = min(g0 + per, groups);
-    int ties = 0;
-    for (int g = g0; g < g1; ++g) {
-        const int i = g * 32 + lane;
-        ties += __popc(__ballot_sync(0xffffffffu, i < n && key_of(i) == prefix));
-    }
-    int total;
-    const int tie0 = warp_offsets<W>(ties, buf, total);
-    // pass 0 counts this warp's freed and moving slots, pass 1 writes them
-    int hole_at = 0, from_at = 0, moves = 0;
-    int2 *list = a.list + (size_t)pair * a.max_moves;
-    for (int pass = 0; pass < 2; ++pass) {
-        int tie = tie0, holes = hole_at, froms = from_at;
+    const bool tied = s_all > want;
+    int total, tie = 0;
+    if (tied) {
+        int ties = 0;
         for (int g = g0; g < g1; ++g) {
             const int i = g * 32 + lane;
-            const uint32_t k = i < n ? key_of(i) : 0u;
+            ties += __popc(__ballot_sync(0xffffffffu, i < n && key_of(i) == prefix));
+        }
+        tie = warp_offsets<W>(ties, buf, total);
+    }
+    for (int g = g0; g < g1; ++g) {
+        const int i = g * 32 + lane;
+        const uint32_t k = i < n ? key_of(i) : 0u;
+        bool keep = i < n && (tied ? k > prefix : k >= prefix);
+        if (tied) {
             const bool eq = i < n && k == prefix;
-            const uint32_t eqs = __ballot_sync(0xffffffffu, eq), below = (1u << lane) - 1u;
-            const bool keep = i < n && (k > prefix || (eq && tie + __popc(eqs & below) < want));
+            const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
+            keep = keep || (eq && tie + __popc(eqs & ((1u << lane) - 1u)) < want);
             tie += __popc(eqs);
-            const bool hole = i < a.budget && !keep, from = i >= a.budget && keep;   // budget < n
-            const uint32_t hb = __ballot_sync(0xffffffffu, hole), fb = __ballot_sync(0xffffffffu, from);
-            if (pass == 1) {
-                const int h = holes + __popc(hb & below), f = froms + __popc(fb & below);
-                if (hole) (h < kSelMoves ? mine[h] : list[h]).y = i;
-                if (from) (f < kSelMoves ? mine[f] : list[f]).x = i;
-            }
-            holes += __popc(hb);
-            froms += __popc(fb);
         }
-        if (pass == 0) {
-            hole_at = warp_offsets<W>(holes, buf, moves);
-            from_at = warp_offsets<W>(froms, buf, moves);  // as many kept behind the budget as freed below it
-        }
+        const uint32_t kept = __ballot_sync(0xffffffffu, keep);
+        if (lane == 0) masks[g] = kept;
+    }
+    __syncthreads();
+    // the lists, a run of groups per thread: freed slots below budget and kept ones behind it are few bits of a mask
+    const int run = (groups + THREADS - 1) / THREADS, r0 = min(tid * run, groups), r1 = min(r0 + run, groups);
+    auto bits = [&](int g, uint32_t &hole, uint32_t &from) {
+        const uint32_t m = masks[g];
+        const int left = a.budget - 32 * g;            // slots of the group below budget (budget < n)
+        const uint32_t below = left <= 0 ? 0u : left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+        hole = ~m & below;
+        from = m & ~below;
+    };
+    int holes = 0, froms = 0;
+    for (int g = r0; g < r1; ++g) {
+        uint32_t h, f;
+        bits(g, h, f);
+        holes += __popc(h);
+        froms += __popc(f);
+    }
+    int hi = holes, fi = froms;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, hi, o), y = __shfl_up_sync(0xffffffffu, fi, o);
+        if (lane >= o) { hi += x; fi += y; }
+    }
+    int moves;
+    int at_h = warp_offsets<W>(__shfl_sync(0xffffffffu, hi, 31), buf, moves) + hi - holes;
+    int at_f = warp_offsets<W>(__shfl_sync(0xffffffffu, fi, 31), buf, moves) + fi - froms;    // as many as freed slots
+    int2 *list = a.list + (size_t)pair * a.max_moves;
+    for (int g = r0; g < r1; ++g) {
+        uint32_t h, f;
+        bits(g, h, f);
+        for (; h; h &= h - 1, ++at_h) (at_h < kSelMoves ? mine[at_h] : list[at_h]).y = 32 * g + __ffs(h) - 1;
+        for (; f; f &= f - 1, ++at_f) (at_f < kSelMoves ? mine[at_f] : list[at_f]).x = 32 * g + __ffs(f) - 1;
     }
     if (tid == 0) a.count[pair] = moves;
     __syncthreads();
     const int here = min(moves, kSelMoves);
-    move_rows(a, pair, [&](int m) { return mine[m]; }, warp, here, W, lane);
     for (int m = tid; m < here; m += THREADS) {
         const size_t at = (size_t)pair * a.max_ctx;
         a.weight_rw[at + mine[m].y] = w[mine[m].x];
         a.slot_pos_rw[at + mine[m].y] = sp[mine[m].x];
     }
+    move_rows(a, pair, [&](int m) { return mine[m]; }, warp, here, W, lane);
 }
 
 constexpr int kMoveWarps = 8;
@@ -243,7 +275,8 @@ template <int THREADS>
 int launch_select(const EvictArgs &a, bool cached, size_t smem, cudaStream_t s) {
     if (smem > 32 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kv_select_kernel<THREADS>,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kSelCacheMax * 4);
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (kSelCacheMax + kSelCacheMax / 32) * 4);
         if (e != cudaSuccess) return (int)e;
     }
     return (int)launch_pdl(kv_select_kernel<THREADS>, dim3((unsigned)a.n_pairs), dim3(THREADS), smem, s, true, a, cached);
@@ -263,7 +296,8 @@ extern "C" {
 size_t li_kv_evict_workspace_size(const li_kv_cache *C, int budget) {
     if (check_kv_cache(C) || C->n_seqs == 0 || budget < 0 || budget > C->max_ctx) return 0;
     const size_t pairs = (size_t)C->n_seqs * C->n_kv_heads;
-    return al256(pairs * sizeof(int32_t)) + al256(pairs * (size_t)moves_max(C, budget) * sizeof(int2));
+    return al256(pairs * sizeof(int32_t)) + al256(pairs * (size_t)moves_max(C, budget) * sizeof(int2)) +
+           (C->max_ctx > kSelCacheMax ? al256(pairs * (((size_t)C->max_ctx + 31) / 32) * 4) : 0);
 }
 
 int li_launch_kv_evict(const li_kv_cache *C, const int32_t *pos, int budget, int n_sink, int n_recent,
@@ -281,13 +315,16 @@ int li_launch_kv_evict(const li_kv_cache *C, const int32_t *pos, int budget, int
     a.Hkv = C->n_kv_heads; a.max_ctx = C->max_ctx; a.budget = budget; a.first_free = (int64_t)C->n_prefix + n_sink; a.n_recent = n_recent;
     a.max_moves = moves_max(C, budget);
     a.count = static_cast<int32_t *>(workspace);
-    a.list = reinterpret_cast<int2 *>(static_cast<char *>(workspace) + al256((size_t)pairs * sizeof(int32_t)));
+    char *ws = static_cast<char *>(workspace) + al256((size_t)pairs * sizeof(int32_t));
+    a.list = reinterpret_cast<int2 *>(ws);
+    a.masks = reinterpret_cast<uint32_t *>(ws + al256((size_t)pairs * (size_t)a.max_moves * sizeof(int2)));
+    a.mask_words = (C->max_ctx + 31) / 32;
     a.k = static_cast<__half *>(C->k); a.v = static_cast<__half *>(C->v);
     a.weight_rw = C->weight; a.slot_pos_rw = C->slot_pos;
     a.n_pairs = pairs;
     const cudaStream_t st = (cudaStream_t)stream;
     const bool cached = C->max_ctx <= kSelCacheMax;
-    const size_t smem = cached ? (size_t)C->max_ctx * 4 : 0;
+    const size_t smem = cached ? ((size_t)C->max_ctx + a.mask_words) * 4 : 0;
     int rc = C->max_ctx < kSelWide ? launch_select<512>(a, cached, smem, st) : launch_select<1024>(a, cached, smem, st);
     if (rc) return rc;
     const int chunks = a.max_moves > kSelMoves ? (a.max_moves - kSelMoves + kMoveChunk - 1) / kMoveChunk : 0;
