@@ -85,7 +85,8 @@ struct KvAttnArgs {
     int *base;                         // [B + 1] first step of every sequence (all kv heads), then the total
     float2 *own_ml;                    // [pairs + own_warps][G]
     float *own_o;                      // [pairs + own_warps][G][128]
-    float *score;                      // [B][Hq][max_ctx], log2 units (weight != nullptr)
+    float *score;                      // [B][Hq][score_stride], log2 units (weight != nullptr)
+    int score_stride;                  // max_ctx rounded up to 4
     bool after_prefix;
     // prefix part
     int n_prefix, rows, n_rt, per_group, n_grp, n_tt;   // rows = B G; row tiles; row tiles per group; groups; tiles
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(kOwnThreads, 1) kv_own_kernel(const __grid_con
                     const int nt = x >> 1, r = x & 1, tok = 8 * nt + 2 * tq + r;
                     s2[x] = (sc[e][nt][r] + sc[e][nt][2 + r]) * c2[e];
                     if (SCORE && 8 * e + g < a.G && tok < left)
-                        a.score[((size_t)cu.s * a.Hq + (size_t)cu.j * a.G + 8 * e + g) * a.max_ctx + t0 + tok] = s2[x];
+                        a.score[((size_t)cu.s * a.Hq + (size_t)cu.j * a.G + 8 * e + g) * a.score_stride + t0 + tok] = s2[x];
                     if (tok >= left) s2[x] = -INFINITY;
                     mx = fmaxf(mx, s2[x]);
                 }
@@ -1044,6 +1045,7 @@ __device__ __forceinline__ float2 piece_ml(const KvAttnArgs &a, const RowPieces 
 }
 
 constexpr int kJoinWarps = 8, kJoinRows = 4;
+constexpr int kJoinRun = kJoinWarps * kWarp * 4;     // slots of a weight block's step
 
 // Rows: wpr neighbouring warps take 4 rows of a kv head, each its share of the
 // pieces; lane l holds row l % 4 and dims 32 i + 4 (l / 4) .. +3, i < 4 (the
@@ -1134,10 +1136,10 @@ __global__ void __launch_bounds__(kJoinWarps * kWarp, 3) kv_join_kernel(const __
         }
         return;
     }
-    // weights of the pair (s, j), every w_chunks-th run of slots
-    const int item = blockIdx.x - a.row_ctas, pair = item / a.w_chunks, chunk = item % a.w_chunks;
-    const int s = pair / a.Hkv, j = pair % a.Hkv, n = own_len(a, s);
-    if (chunk * kJoinWarps * kWarp * 4 >= n) return;
+    // weights of the pair (s, j), every w_chunks-th run of slots, four neighbouring ones a thread
+    const int item = blockIdx.x - a.row_ctas, pair = item / a.w_chunks, chunk = item - pair * a.w_chunks;
+    const int s = pair / a.Hkv, j = pair - s * a.Hkv, n = own_len(a, s);
+    if (chunk * kJoinRun >= n) return;
     for (int gq = warp; gq < a.G; gq += kJoinWarps) {
         const RowPieces x = pieces_of(a, j, s * a.G + gq);
         const int cnt = x.n_pre + x.n_own;
@@ -1158,18 +1160,37 @@ __global__ void __launch_bounds__(kJoinWarps * kWarp, 3) kv_join_kernel(const __
     }
     __syncthreads();
     float *wt = a.weight + (size_t)pair * a.max_ctx;
-    const float *sc = a.score + ((size_t)s * a.Hq + (size_t)j * a.G) * a.max_ctx;
-    const int run = kJoinWarps * kWarp * 4;
-    for (int t0 = chunk * run; t0 < n; t0 += a.w_chunks * run) {
+    const float *sc = a.score + ((size_t)s * a.Hq + (size_t)j * a.G) * a.score_stride;
+    const bool vec = (a.max_ctx & 3) == 0 && ((uintptr_t)a.weight & 15u) == 0;
+    for (int t = chunk * kJoinRun + 4 * tid; t < n; t += a.w_chunks * kJoinRun) {
+        float w[4] = {0.f, 0.f, 0.f, 0.f};
+        const bool whole = vec && t + 4 <= n;
+        if (a.decay != 0.f) {
+            if (whole) {
+                const float4 v = *reinterpret_cast<const float4 *>(wt + t);
+                w[0] = a.decay * v.x; w[1] = a.decay * v.y; w[2] = a.decay * v.z; w[3] = a.decay * v.w;
+            } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int t = t0 + k * kJoinWarps * kWarp + tid;
-            if (t < n) {
-                float w = a.decay == 0.f ? 0.f : a.decay * wt[t];
-                for (int gq = 0; gq < a.G; ++gq)
-                    w = fmaf(ex2(__ldcg(sc + (size_t)gq * a.max_ctx + t) - gm[gq]), gi[gq], w);
-                wt[t] = w;
+                for (int e = 0; e < 4; ++e)
+                    if (t + e < n) w[e] = a.decay * wt[t + e];
             }
+        }
+        // a row of scores has score_stride floats, a multiple of 4: past n it holds nothing, and none of it is kept
+#pragma unroll 4
+        for (int gq = 0; gq < a.G; ++gq) {
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(sc + (size_t)gq * a.score_stride + t));
+            const float m = gm[gq], inv = gi[gq];
+            w[0] = fmaf(ex2(v.x - m), inv, w[0]);
+            w[1] = fmaf(ex2(v.y - m), inv, w[1]);
+            w[2] = fmaf(ex2(v.z - m), inv, w[2]);
+            w[3] = fmaf(ex2(v.w - m), inv, w[3]);
+        }
+        if (whole) {
+            *reinterpret_cast<float4 *>(wt + t) = make_float4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (t + e < n) wt[t + e] = w[e];
         }
     }
 }
@@ -1228,7 +1249,7 @@ size_t plan(const li_kv_cache *C, int n_q_heads, KvAttnArgs *a, size_t *off /* [
     const size_t own_recs = (size_t)pairs + a->own_warps;
     off[1] = at; at += al256(own_recs * a->G * sizeof(float2));
     off[2] = at; at += al256(own_recs * a->G * kKvD * 4);
-    off[3] = at; at += C->weight ? al256((size_t)a->B * a->Hq * a->max_ctx * 4) : 0;
+    off[3] = at; a->score_stride = (int)((a->max_ctx + 3ll) / 4 * 4); at += C->weight ? al256((size_t)a->B * a->Hq * a->score_stride * 4) : 0;
     off[4] = off[5] = at;
     if (a->n_prefix > 0) {
         a->rows = a->B * a->G;
@@ -1331,8 +1352,8 @@ int li_launch_attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_str
     a.row_ctas = (int)((row_blocks + per - 1) / per);
     int64_t blocks = a.row_ctas;
     if (a.weight) {
-        const int run = kJoinWarps * kWarp * 4;
-        int64_t ch = ((int64_t)a.max_ctx + run - 1) / run, cap = ((int64_t)num_sms() * 32 + pairs - 1) / pairs;
+        // blocks per pair: enough for every SM to hold some, since each first joins its pair's sums
+        const int64_t ch = ((int64_t)a.max_ctx + kJoinRun - 1) / kJoinRun, cap = (num_sms() * 4ll + pairs - 1) / pairs;
         a.w_chunks = (int)(ch < cap ? ch : cap);
         blocks += (int64_t)pairs * a.w_chunks;
     }
