@@ -488,6 +488,22 @@ size_t li_attn_kv_workspace_size(const li_kv_cache * C, int n_q_heads);
 int li_launch_attn_kv_decode(const li_kv_cache * C, const float * q, int64_t q_stride, int n_q_heads,
         float scale, float * out, float decay, void * workspace, size_t workspace_bytes, void * stream);
 
+/* One decode step of the gated attention layer (see li_attn_layer) on such a
+ * cache: the input projection, the per-head norms of q and k, their rotation
+ * to position pos[s] by R (NULL: the layer's rope_dim and rope_theta, half
+ * layout, unscaled; R's head_dim is the layer's) and the append to slot
+ * len[s] - 1 as li_launch_kv_append does it, the attention of
+ * li_launch_attn_kv_decode with scale D^-1/2, the output gate and the output
+ * projection. The caller advances len and pos before each step, and shrinks
+ * the cache with li_launch_kv_evict when it likes. A length outside
+ * 1 .. max_ctx appends nothing and li_device_status() reports
+ * LI_ERR_BAD_ARG. Hq / Hkv in 1 .. 16. No counterpart among the reference's
+ * kernels. */
+size_t li_attn_layer_kv_workspace_size(const li_attn_layer * L, const li_kv_cache * C);
+int li_launch_attn_layer_decode_kv(const li_attn_layer * L, const li_rope * R, const li_kv_cache * C,
+        const float * x, float * y, const int32_t * pos, float decay,
+        void * workspace, size_t workspace_bytes, void * stream);
+
 /* Shrinks every sequence of more than `budget` own slots to `budget`, for each
  * kv head by itself. Kept are the slots whose token position (slot_pos) is
  * below n_prefix + n_sink (the first own tokens follow the prefix) or above
@@ -674,6 +690,11 @@ static inline size_t li_attn_kv_workspace_size(const li_kv_cache*C, int h) {(voi
 static inline int li_launch_attn_kv_decode(const li_kv_cache*C, const float*q, int64_t qs, int h, float sc, float*o,
         float d, void*ws, size_t wb, void*s)
         {(void)C;(void)q;(void)qs;(void)h;(void)sc;(void)o;(void)d;(void)ws;(void)wb;(void)s; return LI_ERR_NO_CUDA;}
+static inline size_t li_attn_layer_kv_workspace_size(const li_attn_layer*L, const li_kv_cache*C)
+        {(void)L;(void)C; return 0;}
+static inline int li_launch_attn_layer_decode_kv(const li_attn_layer*L, const li_rope*R, const li_kv_cache*C,
+        const float*x, float*y, const int32_t*p, float d, void*ws, size_t wb, void*s)
+        {(void)L;(void)R;(void)C;(void)x;(void)y;(void)p;(void)d;(void)ws;(void)wb;(void)s; return LI_ERR_NO_CUDA;}
 static inline size_t li_kv_evict_workspace_size(const li_kv_cache*C, int b) {(void)C;(void)b; return 0;}
 static inline int li_launch_kv_evict(const li_kv_cache*C, const int32_t*p, int b, int ns, int nr, void*ws, size_t wb,
         void*s)

@@ -52,7 +52,20 @@
  *                               eps as floats. Needs a workspace of
  *                               li_ggml_workspace_size(node) bytes.
  *
- * Every tensor must be contiguous (f32: nb[0] = 4 and nb[i+1] = nb[i] *
+ *   LI_GGML_OP_ROPE             rotary positions (ggml ROPE) -> li_launch_rope;
+ *                               src0 x [D, heads, tokens] and dst the same
+ *                               shape and type, f32, f16 or bf16, each head's
+ *                               D values contiguous, any nb[1] and nb[2]
+ *                               (multiples of the element size), ne[3] = 1;
+ *                               src1 positions i32 [tokens]; src2 frequency
+ *                               divisors f32 [rope dims / 2] or NULL. ggml's op
+ *                               parameters: [1] = rope dims, [2] = mode (0:
+ *                               interleaved pairs, 2: halves), [4] = original
+ *                               context, as floats [5] = base, [6] = frequency
+ *                               scale, [7] = extrapolation mix, [8] = magnitude,
+ *                               [9], [10] = beta fast, slow (see li_rope).
+ *
+ * Every tensor of the other nodes must be contiguous (f32: nb[0] = 4 and nb[i+1] = nb[i] *
  * ne[i]; quantized: nb[1] = the row size of ne[0] values, higher strides
  * contiguous over rows). Returns LI_OK, LI_ERR_BAD_ARG (null node, source or
  * data), LI_ERR_UNSUPPORTED (op or type), LI_ERR_BAD_SHAPE (shapes that do
@@ -74,7 +87,9 @@ enum li_ggml_type {
     LI_GGML_TYPE_F32  = 0,
     LI_GGML_TYPE_F16  = 1,
     LI_GGML_TYPE_Q8_0 = 8,
-    LI_GGML_TYPE_Q4_K = 12
+    LI_GGML_TYPE_Q4_K = 12,
+    LI_GGML_TYPE_I32  = 26,
+    LI_GGML_TYPE_BF16 = 30
 };
 
 enum li_ggml_op {
@@ -82,7 +97,8 @@ enum li_ggml_op {
     LI_GGML_OP_MUL_MAT = 1,
     LI_GGML_OP_FUSED_UP_GATE = 2,
     LI_GGML_OP_FUSED_RMS_SILU_GATE = 3,
-    LI_GGML_OP_DELTANET_DECODE = 4
+    LI_GGML_OP_DELTANET_DECODE = 4,
+    LI_GGML_OP_ROPE = 5
 };
 
 #define LI_GGML_MAX_DIMS 4

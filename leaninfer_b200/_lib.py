@@ -170,6 +170,10 @@ _SIGS = {
     "li_attn_kv_workspace_size": (c_size_t, [POINTER(KvCache), c_int]),
     "li_launch_attn_kv_decode": (
         c_int, [POINTER(KvCache), c_void_p, c_int64, c_int, c_float, c_void_p, c_float, c_void_p, c_size_t, c_void_p]),
+    "li_attn_layer_kv_workspace_size": (c_size_t, [POINTER(AttnLayer), POINTER(KvCache)]),
+    "li_launch_attn_layer_decode_kv": (
+        c_int, [POINTER(AttnLayer), POINTER(RopeParams), POINTER(KvCache), c_void_p, c_void_p, c_void_p, c_float,
+                c_void_p, c_size_t, c_void_p]),
     "li_kv_evict_workspace_size": (c_size_t, [POINTER(KvCache), c_int]),
     "li_launch_kv_evict": (
         c_int, [POINTER(KvCache), c_void_p, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),

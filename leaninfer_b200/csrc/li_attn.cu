@@ -26,6 +26,7 @@
 //   out-projection the quantized GEMV or tcgen05 GEMM again.
 // HBM-bound: a step reads each cached token's K and V row once per kv head.
 #include "li_common.cuh"
+#include "li_kv.cuh"
 #include "li_qgemv.cuh"
 #include "li_tc.cuh"
 #include "li_tcgemm.cuh"
@@ -124,6 +125,86 @@ __global__ void __launch_bounds__(256) attn_prep_kernel(AttnArgs a, int B) {
             a.k_cache[off + lane + 32 * m] = __float2half_rn(v[m]);
             a.v_cache[off + lane + 32 * m] = __float2half_rn(vs[lane + 32 * m]);
         }
+    }
+}
+
+// The same on a managed cache (li_kv_cache): rotation by the caller's
+// parameters to position pos[s], append to slot len[s] - 1, whose weight and
+// position are set. Warp per (sequence, head slot), as above; pair values are
+// exchanged through shared memory, so that either pair layout does.
+struct KvPrepArgs {
+    RopeArgs r;
+    float *proj;
+    int NP, Hq, Hkv, max_ctx, B;
+    const float *q_norm_w, *k_norm_w;
+    float eps;
+    const int32_t *pos, *len;
+    __half *k, *v;
+    float *weight;
+    int32_t *slot_pos;
+};
+
+__global__ void __launch_bounds__(256) kv_prep_kernel(const __grid_constant__ KvPrepArgs a) {
+    __shared__ float vec[8][kD];
+    grid_dep_wait();
+    grid_dep_launch_dependents();
+    const int wi = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    const int slots = a.Hq + a.Hkv;
+    const int gw = blockIdx.x * 8 + wi;
+    if (gw >= a.B * slots) return;
+    const int s = gw / slots, hs = gw % slots, pos = a.pos[s];
+    const bool is_q = hs < a.Hq;
+    const int j = hs - a.Hq, slot = a.len[s] - 1;
+    if (!is_q && (slot < 0 || slot >= a.max_ctx)) {
+        // no slot for this token: nothing is written, the device flag is raised
+        if (j == 0 && lane == 0) atomicExch(&g_device_error, LI_ERR_BAD_ARG);
+        return;
+    }
+    float *ps = a.proj + (size_t)s * a.NP;
+    float *src = is_q ? ps + (size_t)hs * kD : ps + (size_t)2 * a.Hq * kD + (size_t)j * kD;
+    const float *w = is_q ? a.q_norm_w : a.k_norm_w;
+    float v[4];
+    float sq = 0.f;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+        v[m] = src[lane + 32 * m];
+        sq = fmaf(v[m], v[m], sq);
+    }
+    if (w) {
+        const float r = rsqrtf(warp_sum(sq) / (float)kD + a.eps);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) v[m] = v[m] * w[lane + 32 * m] * r;
+    }
+#pragma unroll
+    for (int m = 0; m < 4; ++m) vec[wi][lane + 32 * m] = v[m];
+    __syncwarp();
+    const int half = a.r.rope_dim / 2;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+        const int i = lane + 32 * m;
+        if (i < a.r.rope_dim) {
+            const bool hl = a.r.layout == LI_ROPE_HALF;
+            const int f = hl ? (i < half ? i : i - half) : i >> 1;              // pair
+            const bool first = hl ? i < half : !(i & 1);
+            const float2 c = rope_cos_sin(a.r, pos, f);
+            const float x1 = vec[wi][hl ? f : 2 * f], x2 = vec[wi][hl ? f + half : 2 * f + 1];
+            v[m] = first ? x1 * c.x - x2 * c.y : x2 * c.x + x1 * c.y;
+        }
+    }
+    if (is_q) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) src[lane + 32 * m] = v[m];
+    } else {
+        const size_t off = (((size_t)s * a.max_ctx + slot) * a.Hkv + j) * kD;
+        const float *vs = ps + (size_t)2 * a.Hq * kD + (size_t)a.Hkv * kD + (size_t)j * kD;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            a.k[off + lane + 32 * m] = __float2half_rn(v[m]);
+            a.v[off + lane + 32 * m] = __float2half_rn(vs[lane + 32 * m]);
+        }
+        const size_t at = ((size_t)s * a.Hkv + j) * a.max_ctx + slot;
+        if (lane == 0 && a.weight) a.weight[at] = 0.f;
+        if (lane == 0 && a.slot_pos) a.slot_pos[at] = pos;
     }
 }
 
@@ -943,4 +1024,73 @@ int li::attn_layer_decode_residual(const li_attn_layer *L, const float *x, float
                                    size_t workspace_bytes, void *stream) {
     return attn_layer_decode(L, x, y, k_cache, v_cache, pos, n_seqs, max_ctx, workspace, workspace_bytes, stream,
                              true);
+}
+
+// ---------------------------------------------------------------------------
+// The layer on a managed cache
+// ---------------------------------------------------------------------------
+static int check_layer_kv(const li_attn_layer *L, const li_kv_cache *C) {
+    if (const int rc = check_kv_cache(C)) return rc;
+    if (!L || !L->w_in || !L->w_out) return LI_ERR_BAD_ARG;
+    if (L->head_dim != kD) return LI_ERR_UNSUPPORTED;
+    if (L->n_q_heads <= 0 || L->n_kv_heads != C->n_kv_heads || L->n_q_heads % L->n_kv_heads) return LI_ERR_BAD_SHAPE;
+    if (L->n_q_heads / L->n_kv_heads > 16) return LI_ERR_UNSUPPORTED;
+    if ((L->w_in_type != LI_WTYPE_Q4_K && L->w_in_type != LI_WTYPE_Q8_0) ||
+        (L->w_out_type != LI_WTYPE_Q4_K && L->w_out_type != LI_WTYPE_Q8_0))
+        return LI_ERR_UNSUPPORTED;
+    return 0;
+}
+
+extern "C" size_t li_attn_layer_kv_workspace_size(const li_attn_layer *L, const li_kv_cache *C) {
+    if (check_layer_kv(L, C) || C->n_seqs == 0) return 0;
+    const size_t attn = li_attn_kv_workspace_size(C, L->n_q_heads);
+    return attn ? attn_ws_layout(L, C->n_seqs, 1).total + attn : 0;
+}
+
+extern "C" int li_launch_attn_layer_decode_kv(const li_attn_layer *L, const li_rope *R, const li_kv_cache *C,
+                                              const float *x, float *y, const int32_t *pos, float decay,
+                                              void *workspace, size_t workspace_bytes, void *stream) {
+    if (const int rc = check_layer_kv(L, C)) return rc;
+    if (!x || !y || !pos || !(decay >= 0.0f)) return LI_ERR_BAD_ARG;
+    KvPrepArgs a = {};
+    li_rope from_layer = {};
+    if (!R) {
+        from_layer.layout = LI_ROPE_HALF;
+        from_layer.head_dim = kD;
+        from_layer.rope_dim = L->rope_dim;
+        from_layer.theta = L->rope_dim > 0 ? L->rope_theta : 2.0f;
+        from_layer.freq_scale = from_layer.attn_factor = 1.0f;
+        R = &from_layer;
+    }
+    if (const int rc = rope_args(R, &a.r)) return rc;
+    if (R->head_dim != kD) return LI_ERR_BAD_SHAPE;
+    if (!aligned16(x) || !aligned16(y) || (L->in_norm_w && !aligned16(L->in_norm_w)) || ((uintptr_t)pos & 3u))
+        return LI_ERR_MISALIGNED;
+    const int n = C->n_seqs, Hq = L->n_q_heads, Hkv = L->n_kv_heads, NP = 2 * Hq * kD + 2 * Hkv * kD;
+    if (n == 0) return 0;
+    const AttnWs lay = attn_ws_layout(L, n, 1);
+    const size_t need = li_attn_layer_kv_workspace_size(L, C);
+    if (need == 0) return LI_ERR_BAD_SHAPE;
+    if (!workspace || workspace_bytes < need) return LI_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return LI_ERR_MISALIGNED;
+    char *ws = (char *)workspace;
+    const cudaStream_t s = (cudaStream_t)stream;
+    const bool simt = attn_simt(L, n);
+    float *proj = reinterpret_cast<float *>(ws + lay.proj), *og = reinterpret_cast<float *>(ws + lay.og);
+    int rc;
+    if ((rc = project(simt, L->w_in_type, L->w_in, L->hidden, NP, x, L->in_norm_w, L->in_norm_eps, proj, n, ws, lay,
+                      true, false, s)))
+        return rc;
+    a.proj = proj; a.NP = NP; a.Hq = Hq; a.Hkv = Hkv; a.max_ctx = C->max_ctx; a.B = n;
+    a.q_norm_w = L->q_norm_w; a.k_norm_w = L->k_norm_w; a.eps = L->qk_norm_eps;
+    a.pos = pos; a.len = C->len;
+    a.k = static_cast<__half *>(C->k); a.v = static_cast<__half *>(C->v);
+    a.weight = C->weight; a.slot_pos = C->slot_pos;
+    const int64_t warps = (int64_t)n * (Hq + Hkv);
+    if (warps > (1ll << 30)) return LI_ERR_BAD_SHAPE;
+    if ((rc = (int)launch_pdl(kv_prep_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, s, true, a))) return rc;
+    if ((rc = attn_kv_decode(C, proj, NP, Hq, 1.0f / sqrtf((float)kD), og, decay, proj + (size_t)Hq * kD, NP,
+                             ws + lay.total, workspace_bytes - lay.total, stream)))
+        return rc;
+    return project(simt, L->w_out_type, L->w_out, Hq * kD, L->hidden, og, nullptr, 0.f, y, n, ws, lay, false, true, s);
 }

@@ -180,6 +180,39 @@ int li_ggml_compute_forward(const li_ggml_tensor *node, void *workspace, size_t 
                                                (float *)node->src[1]->data, (float *)node->src[2]->data, n,
                                                workspace, workspace_bytes, stream);
     }
+    case LI_GGML_OP_ROPE: {
+        const li_ggml_tensor *x = node->src[0], *pos = node->src[1], *ff = node->src[2];
+        if (!x || !pos || !x->data || !pos->data) return LI_ERR_BAD_ARG;
+        const int es = x->type == LI_GGML_TYPE_F32 ? 4
+                       : x->type == LI_GGML_TYPE_F16 || x->type == LI_GGML_TYPE_BF16 ? 2 : 0;
+        if (!es || node->type != x->type || pos->type != LI_GGML_TYPE_I32) return LI_ERR_UNSUPPORTED;
+        const int mode = node->op_params[2];
+        if (mode != 0 && mode != 2) return LI_ERR_UNSUPPORTED;
+        if (!dims_ok(x) || x->ne[3] != 1 || pos->ne[0] != x->ne[2] || rows_of(pos) != 1 || pos->nb[0] != 4)
+            return LI_ERR_BAD_SHAPE;
+        for (int i = 0; i < LI_GGML_MAX_DIMS; ++i)
+            if (node->ne[i] != x->ne[i]) return LI_ERR_BAD_SHAPE;
+        for (const li_ggml_tensor *t : {x, node})
+            if (t->nb[0] != (size_t)es || t->nb[1] % es || t->nb[2] % es) return LI_ERR_BAD_SHAPE;
+        if (!fits_int(x->ne[0]) || !fits_int(x->ne[1]) || !fits_int(x->ne[2])) return LI_ERR_BAD_SHAPE;
+        li_rope R;
+        std::memset(&R, 0, sizeof(R));
+        R.layout = mode == 2 ? LI_ROPE_HALF : LI_ROPE_INTERLEAVED;
+        R.head_dim = (int)x->ne[0];
+        R.rope_dim = node->op_params[1];
+        R.n_ctx_orig = node->op_params[4];
+        R.theta = param_f32(node, 5);
+        R.freq_scale = param_f32(node, 6);
+        R.ext_factor = param_f32(node, 7);
+        R.attn_factor = param_f32(node, 8);
+        R.beta_fast = param_f32(node, 9);
+        R.beta_slow = param_f32(node, 10);
+        if (ff && (!ff->data || !f32_vector(ff, R.rope_dim / 2))) return LI_ERR_BAD_SHAPE;
+        R.freq_factors = ff ? (const float *)ff->data : nullptr;
+        return li_launch_rope(&R, x->type, x->data, node->data, (const int32_t *)pos->data, (int)x->ne[2],
+                              (int)x->ne[1], (int64_t)(x->nb[2] / es), (int64_t)(x->nb[1] / es),
+                              (int64_t)(node->nb[2] / es), (int64_t)(node->nb[1] / es), 0, stream);
+    }
     default:
         return LI_ERR_UNSUPPORTED;
     }

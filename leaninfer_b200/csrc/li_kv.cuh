@@ -51,4 +51,10 @@ __device__ __forceinline__ float2 rope_cos_sin(const RopeArgs &a, int pos, int i
     return make_float2(cs * a.mag, sn * a.mag);
 }
 
+// li_launch_attn_kv_decode, with an optional output gate: out = o *
+// sigmoid(gate), gate [n_seqs][gate_stride] laid out as q (nullptr: none).
+int attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_stride, int n_q_heads, float scale, float *out,
+                   float decay, const float *gate, int64_t gate_stride, void *workspace, size_t workspace_bytes,
+                   void *stream);
+
 }  // namespace li

@@ -80,6 +80,8 @@ struct KvAttnArgs {
     float qsign;                       // sign of scale, applied to q
     float decay;
     float *out, *weight;
+    const float *gate;                 // sigmoid(gate) times the output, or nullptr
+    int64_t gate_stride;
     // own part
     int own_warps;                     // warps of the kv_own grid
     int *base;                         // [B + 1] first step of every sequence (all kv heads), then the total
@@ -1131,8 +1133,15 @@ __global__ void __launch_bounds__(kJoinWarps * kWarp, 3) kv_join_kernel(const __
             const int s = row / a.G;
             float4 *d = reinterpret_cast<float4 *>(a.out + ((size_t)s * a.Hq + (size_t)j * a.G + row - s * a.G) * kKvD) + xq;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                d[8 * k] = make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv);
+            for (int k = 0; k < 4; ++k) {
+                float4 v = make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv);
+                if (a.gate) {
+                    const float4 gt = reinterpret_cast<const float4 *>(
+                        a.gate + s * a.gate_stride + ((size_t)j * a.G + row - s * a.G) * kKvD)[xq + 8 * k];
+                    v.x *= sigmoid(gt.x); v.y *= sigmoid(gt.y); v.z *= sigmoid(gt.z); v.w *= sigmoid(gt.w);
+                }
+                d[8 * k] = v;
+            }
         }
         return;
     }
@@ -1249,7 +1258,8 @@ size_t plan(const li_kv_cache *C, int n_q_heads, KvAttnArgs *a, size_t *off /* [
     const size_t own_recs = (size_t)pairs + a->own_warps;
     off[1] = at; at += al256(own_recs * a->G * sizeof(float2));
     off[2] = at; at += al256(own_recs * a->G * kKvD * 4);
-    off[3] = at; a->score_stride = (int)((a->max_ctx + 3ll) / 4 * 4); at += C->weight ? al256((size_t)a->B * a->Hq * a->score_stride * 4) : 0;
+    a->score_stride = (a->max_ctx + 3) / 4 * 4;
+    off[3] = at; at += C->weight ? al256((size_t)a->B * a->Hq * a->score_stride * 4) : 0;
     off[4] = off[5] = at;
     if (a->n_prefix > 0) {
         a->rows = a->B * a->G;
@@ -1296,6 +1306,14 @@ size_t li_attn_kv_workspace_size(const li_kv_cache *C, int n_q_heads) {
 
 int li_launch_attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_stride, int n_q_heads, float scale,
                              float *out, float decay, void *workspace, size_t workspace_bytes, void *stream) {
+    return attn_kv_decode(C, q, q_stride, n_q_heads, scale, out, decay, nullptr, 0, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"
+
+int li::attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_stride, int n_q_heads, float scale, float *out,
+                       float decay, const float *gate, int64_t gate_stride, void *workspace, size_t workspace_bytes,
+                       void *stream) {
     if (const int rc = check_kv_cache(C)) return rc;
     if (!q || !out || n_q_heads <= 0 || !(decay >= 0.0f)) return LI_ERR_BAD_ARG;
     if (n_q_heads % C->n_kv_heads) return LI_ERR_BAD_SHAPE;
@@ -1315,6 +1333,7 @@ int li_launch_attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_str
     a.len = C->len;
     a.cscale = fabsf(scale) * kLog2e; a.qsign = scale < 0.f ? -1.f : 1.f;
     a.decay = decay; a.out = out; a.weight = C->weight;
+    a.gate = gate; a.gate_stride = gate_stride;
     a.base = reinterpret_cast<int *>(ws + off[0]);
     a.own_ml = reinterpret_cast<float2 *>(ws + off[1]);
     a.own_o = reinterpret_cast<float *>(ws + off[2]);
@@ -1360,5 +1379,3 @@ int li_launch_attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_str
     if (blocks > 0x7fffffff) return LI_ERR_BAD_SHAPE;
     return (int)launch_pdl(kv_join_kernel, dim3((unsigned)blocks), dim3(kJoinWarps * kWarp), 0, st, true, a);
 }
-
-}  // extern "C"

@@ -11,8 +11,8 @@ import torch
 from . import _lib
 from ._lib import GgmlTensor
 
-F32, F16, Q8_0, Q4_K = 0, 1, 8, 12
-OP_MUL_MAT, OP_FUSED_UP_GATE, OP_FUSED_RMS_SILU_GATE, OP_DELTANET_DECODE = 1, 2, 3, 4
+F32, F16, Q8_0, Q4_K, I32, BF16 = 0, 1, 8, 12, 26, 30
+OP_MUL_MAT, OP_FUSED_UP_GATE, OP_FUSED_RMS_SILU_GATE, OP_DELTANET_DECODE, OP_ROPE = 1, 2, 3, 4, 5
 _BLOCK = {Q8_0: (32, 34), Q4_K: (256, 144)}
 
 
@@ -27,6 +27,19 @@ def f32_desc(t: torch.Tensor) -> GgmlTensor:
     for i in range(4):
         d.ne[i] = int(dims[i])
         d.nb[i] = int(strides[i]) * 4
+    d.data = t.data_ptr()
+    return d
+
+
+def desc(t: torch.Tensor) -> GgmlTensor:
+    """Descriptor of an fp32, fp16, bf16 or int32 tensor, strided as it is."""
+    d = GgmlTensor()
+    d.type = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int32: I32}[t.dtype]
+    dims = list(reversed(t.shape)) + [1] * (4 - t.dim())
+    strides = list(reversed(t.stride())) + [t.numel()] * (4 - t.dim())
+    for i in range(4):
+        d.ne[i] = int(dims[i])
+        d.nb[i] = int(strides[i]) * t.element_size()
     d.data = t.data_ptr()
     return d
 

@@ -321,6 +321,23 @@ class AttnLayerDecode:
             ws.numel(), _stream()), "li_launch_attn_layer_decode")
         return y
 
+    def step_kv(self, x, y, cache: "KVCache", pos, rope: "Rope | None" = None, decay: float = 1.0, workspace=None):
+        """One decode step on a managed cache: the new token of sequence s, at
+        position pos[s] (int32), goes to slot cache.len[s] - 1; rope defaults
+        to the layer's own parameters."""
+        _on(cache.index, x, y, pos, workspace)
+        if x.shape != (cache.n_seqs, self.L.hidden) or y.shape != x.shape or x.dtype != y.dtype or \
+                x.dtype != torch.float32:
+            raise ValueError(f"x, y: expected fp32 [{cache.n_seqs}, {self.L.hidden}]")
+        lib, L = _lib.load(), self.L
+        ws = workspace if workspace is not None else cache._workspace(
+            ("layer", L.hidden, L.n_q_heads, L.w_in_type, L.w_out_type), lambda: int(lib.li_attn_layer_kv_workspace_size(ctypes.byref(self.L), cache.ref)))
+        check(lib.li_launch_attn_layer_decode_kv(
+            ctypes.byref(self.L), rope.ref if rope is not None else None, cache.ref, _p(x), _p(y),
+            _index(pos, cache.n_seqs, "pos"), decay, ws.data_ptr(), ws.numel(), _stream()),
+            "li_launch_attn_layer_decode_kv")
+        return y
+
 
 # --------------------------------------------------------------------------
 # Rotary positions and the managed KV cache

@@ -185,3 +185,75 @@ def test_wrappers_refuse_cpu_tensors_and_wrong_shapes(lib):
         ops.KVCache(k, k.clone(), n, k_prefix=k[0])
     with pytest.raises(ValueError, match="weight"):
         ops.KVCache(k, k.clone(), n, weight=torch.zeros(2, 2, 7))
+
+
+def _layer(**kw):
+    from leaninfer_b200._lib import AttnLayer
+    d = dict(hidden=1024, n_q_heads=8, n_kv_heads=2, head_dim=128, rope_dim=64, w_in_type=12, w_out_type=12,
+             rope_theta=1e6, in_norm_eps=1e-6, qk_norm_eps=1e-6, w_in=P, w_out=P)
+    d.update(kw)
+    return AttnLayer(**d)
+
+
+def test_layer_on_a_managed_cache_arguments(lib):
+    c = _cache()
+    need = lib.li_attn_layer_kv_workspace_size(ctypes.byref(_layer()), ctypes.byref(c))
+    assert need > lib.li_attn_kv_workspace_size(ctypes.byref(c), 8) > 0
+
+    def call(L=None, R=None, C=c, x=P, y=P, pos=P, decay=1.0, ws=P, wb=need):
+        return lib.li_launch_attn_layer_decode_kv(ctypes.byref(L or _layer()), ctypes.byref(R) if R else None,
+                                                  ctypes.byref(C), x, y, pos, decay, ws, wb, None)
+
+    for change, want in ((dict(w_in=None), BAD_ARG), (dict(w_out=None), BAD_ARG), (dict(head_dim=64), UNSUPPORTED),
+                         (dict(n_kv_heads=4), BAD_SHAPE), (dict(n_q_heads=7), BAD_SHAPE), (dict(n_q_heads=34), UNSUPPORTED),
+                         (dict(w_in_type=2), UNSUPPORTED), (dict(w_out_type=0), UNSUPPORTED), (dict(rope_dim=63), BAD_SHAPE),
+                         (dict(rope_theta=0.5), BAD_ARG), (dict(in_norm_w=P + 4), MISALIGNED)):
+        assert call(L=_layer(**change)) == want, change
+    assert call(x=None) == BAD_ARG and call(y=None) == BAD_ARG and call(pos=None) == BAD_ARG
+    assert call(decay=-1.0) == BAD_ARG
+    assert call(R=_rope(head_dim=64)) == BAD_SHAPE and call(R=_rope(theta=0.0)) == BAD_ARG
+    assert call(x=P + 4) == MISALIGNED and call(pos=P + 2) == MISALIGNED and call(ws=P + 8) == MISALIGNED
+    assert call(ws=None) == WORKSPACE and call(wb=need - 1) == WORKSPACE
+    for change, want in CACHE_FAULTS:
+        assert call(C=_cache(**change)) == want, change
+    c.n_seqs = 0
+    assert call() == 0
+
+
+def test_rope_node_checks(lib):
+    """The ggml ROPE node's checks; a node that passes them reaches the entry's
+    own (here: a head_dim beyond its limit)."""
+    from leaninfer_b200 import ggml
+    from leaninfer_b200._lib import GgmlTensor
+
+    def t(kind, ne, es):
+        d = GgmlTensor()
+        d.type, d.data = kind, P
+        s = es
+        for i in range(4):
+            d.ne[i] = ne[i] if i < len(ne) else 1
+            d.nb[i] = s
+            s *= d.ne[i]
+        return d
+
+    def run(x=None, pos=None, ff=None, out=None, **kw):
+        p = [0, kw.get("dims", 64), kw.get("mode", 2), 0, 4096, 1e4, 1.0, 0.0, 1.0, 32.0, 1.0]
+        x = x or t(ggml.F32, [128, 4, 5], 4)
+        nd = ggml.node(ggml.OP_ROPE, out or t(x.type, list(x.ne), x.nb[0]), [x, pos or t(ggml.I32, [5], 4), ff], p)
+        return lib.li_ggml_compute_forward(ctypes.byref(nd), None, 0, None)
+
+    assert run(mode=1) == UNSUPPORTED and run(mode=8) == UNSUPPORTED
+    assert run(x=t(ggml.Q8_0, [128, 4, 5], 34)) == UNSUPPORTED
+    assert run(pos=t(ggml.F32, [5], 4)) == UNSUPPORTED
+    assert run(out=t(ggml.F16, [128, 4, 5], 2)) == UNSUPPORTED
+    assert run(pos=t(ggml.I32, [4], 4)) == BAD_SHAPE
+    assert run(x=t(ggml.F32, [128, 4, 5, 2], 4)) == BAD_SHAPE
+    assert run(out=t(ggml.F32, [128, 4, 6], 4)) == BAD_SHAPE
+    assert run(ff=t(ggml.F32, [64], 4)) == BAD_SHAPE
+    odd = t(ggml.F32, [128, 4, 5], 4)
+    odd.nb[1] += 2
+    assert run(x=odd) == BAD_SHAPE
+    assert run(dims=130) == BAD_SHAPE and run(x=t(ggml.F32, [514, 4, 5], 4)) == BAD_SHAPE
+    gone = t(ggml.I32, [5], 4)
+    gone.data = None
+    assert run(pos=gone) == BAD_ARG
