@@ -624,13 +624,13 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 float4 *d = reinterpret_cast<float4 *>(a.pre_o + ((size_t)(p + c) * 2 + b) * kPreRows * kKvD) + r;
                 const float m_old = b ? m_rec1 : m_rec0;
                 const bool again = live && m_old != -INFINITY;
-                float4 old[8];
-                auto fetch = [&](int x) {
+                float4 old[2][8];                                  // the record's values, a round ahead
+                auto fetch = [&](float4 (&o)[8], int x) {
 #pragma unroll
                     for (int y = 0; y < 8; ++y)
-                        old[y] = again ? __ldcg(d + (8 * x + y) * kPreRows) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        o[y] = again ? __ldcg(d + (8 * x + y) * kPreRows) : make_float4(0.f, 0.f, 0.f, 0.f);
                 };
-                fetch(0);
+                fetch(old[0], 0);
                 ok = __all_sync(0xffffffffu, wait_or_abort(&o_full[b], (po >> b) & 1u, abort_flag) &&
                                                  wait_or_abort(&m_full[b], (po >> b) & 1u, abort_flag));
                 if (!ok) break;
@@ -639,25 +639,30 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 const float m = m_of[b * kPreRows + r], f = again ? ex2(m_old - m) : 0.f;
                 (b ? m_rec1 : m_rec0) = m;
 #pragma unroll 1
-                for (int x = 0; x < 4; ++x) {
-                    uint32_t v[32];
-                    tmem_ld32_nowait(lane_base + 128u * b + 32u * x, v);
-                    tmem_wait_ld();
-                    if (x == 3) {                                  // o may be overwritten
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&o_read[b]);
-                    }
-                    if (live)
+                for (int x0 = 0; x0 < 4; x0 += 2)
 #pragma unroll
-                        for (int y = 0; y < 8; ++y)
-                            __stcg(d + (8 * x + y) * kPreRows,
-                                   make_float4(fmaf(old[y].x, f, __uint_as_float(v[4 * y])),
-                                               fmaf(old[y].y, f, __uint_as_float(v[4 * y + 1])),
-                                               fmaf(old[y].z, f, __uint_as_float(v[4 * y + 2])),
-                                               fmaf(old[y].w, f, __uint_as_float(v[4 * y + 3]))));
-                    if (x < 3) fetch(x + 1);
-                }
+                    for (int e = 0; e < 2; ++e) {
+                        const int x = x0 + e;
+                        uint32_t v[32];
+                        tmem_ld32_nowait(lane_base + 128u * b + 32u * x, v);
+                        if (x < 3) fetch(old[e ^ 1], x + 1);
+                        tmem_wait_ld();
+                        if (x == 3) {                              // o may be overwritten
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&o_read[b]);
+                        }
+                        if (live)
+#pragma unroll
+                            for (int y = 0; y < 8; ++y) {
+                                const float4 w = old[e][y];
+                                __stcg(d + (8 * x + y) * kPreRows,
+                                       make_float4(fmaf(w.x, f, __uint_as_float(v[4 * y])),
+                                                   fmaf(w.y, f, __uint_as_float(v[4 * y + 1])),
+                                                   fmaf(w.z, f, __uint_as_float(v[4 * y + 2])),
+                                                   fmaf(w.w, f, __uint_as_float(v[4 * y + 3]))));
+                            }
+                    }
             }
         }
     } else if (warp >= 8) {
@@ -788,14 +793,15 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                     for (int x = 0; x < 8; ++x)
                         umma_f16_ta(to, ts + 64u + (x < 4 ? 16u : 0u) + 32u * ((x & 3) >> 1) + 8u * (x & 1),
                                     vd + 512u + 128u * (x & 3), id_o, 1u);
+                    // at once, not behind the scores: the next K tile but one takes this slot, and the ring is short
+                    release(vp.slot);
                     // o goes to the record: the buffer's last unit, or kPreFlush of them summed
                     if (!more || sum_ends(u >> 1, b)) umma_commit(&o_full[b]);
                     // an odd piece ends with buffer 0, which begins the next
                     if (more) scores(k0 + (uint64_t)(kp.slot * (kPreSlotBytes >> 4)), true);
                     else if (u + 1 < U || b == 1) pass();
-                    if (more) umma_commit(&s_full[b]);
-                    release(vp.slot);
                     if (more) {
+                        umma_commit(&s_full[b]);
                         release(kp.slot);
                         advance(vp, g.nt == 2 ? 2 : v_place(t + 2, 1, n) - v_place(t, 1, n));
                     }
