@@ -67,7 +67,8 @@ constexpr uint32_t kPreSlotBytes = kPreTok * kKvD * 2;      // 128 tokens of K o
 constexpr uint32_t kPreQBytes = 2 * kPreRows * kKvD * 2;    // a row tile's hi and lo: 64 KB
 constexpr int kPreSlots2 = 3, kPreSlots1 = 5;  // ring slots beside two / one row tiles of q
 constexpr int kPreFlush = 4;                   // token tiles summed in tensor memory before they join the record
-constexpr size_t kPreSmem = 1024 + 2 * kPreQBytes + kPreSlots2 * kPreSlotBytes + 256 + 2 * kPreRows * 4;
+constexpr size_t kPreSmem = 1024 + 2 * kPreQBytes + kPreSlots2 * kPreSlotBytes + 256 + 3 * kPreRows * 4;
+static_assert(kPreSmem <= 227 * 1024, "shared memory");
 static_assert(2 * kPreQBytes + kPreSlots2 * kPreSlotBytes == kPreQBytes + kPreSlots1 * kPreSlotBytes, "ring");
 
 struct KvAttnArgs {
@@ -563,6 +564,7 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(o_read + 2);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
     float *m_of = reinterpret_cast<float *>(bars + 32);            // [buffer][row]: the maximum a sum of P V refers to
+    float *c_of = m_of + 2 * kPreRows;                             // [row]: the scores' scale, where both buffers have it
     const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
     const int slots = a.slots;
     if (tid == 0) {
@@ -815,7 +817,7 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         const int b = warp >> 2, r = tid & 127;
         const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t sb = lane_base + 128u * b, ob = lane_base + 256u + 128u * b;
-        uint32_t ps = 0, pr = 1;                                   // phases of s_full, o_read (before)
+        uint32_t ps = 0, pr = 1, pq = 0;                           // phases of s_full, o_read (before), q_full
         bool stop = false;
         for (int p = p0; !stop && p < p_end; ++p) {
             const Group g = group_at(a, p);
@@ -824,70 +826,76 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             tiles_of(a, g.base, g.nt, lo, hi, t0, t1);
             const int n = t1 - t0;
             if (n <= 0) continue;
-            // this warp's 32 rows of q: scaled, split and stored as the operand's rows. Eight lanes take a row
-            // (128 contiguous bytes a load), four rows a step, two steps' loads in flight.
+            // This warp's 32 rows of q, scaled and split into the operand's rows. They are copied as they are
+            // first, all in flight at once: row r's 512 bytes are the 128-byte rows r of the operand's four blocks
+            // (hi and lo, 64 dims each), so that each row is then converted in its own place. One row tile: buffer
+            // 0's warps do it for both.
             const int tile0 = (g.rt + (g.nt == 2 ? b : 0)) * kPreRows, row = tile0 + r;
             const bool live = row < a.rows;
             float c2 = 0.f;
-            {
-                const int sub = lane >> 3, l8 = lane & 7;
-                const bool put = g.nt == 2 || b == 0;
-                uint8_t *qd = qbuf + (g.nt == 2 ? (size_t)b * kPreQBytes : 0) + (l8 & 1) * 8;
-                int rr = tile0 + 32 * (warp & 3) + sub, s = rr / a.G, h = rr - s * a.G;      // the row to fetch next
-                float4 x[2][4];
-                auto fetch = [&](float4 (&v)[4]) {
-                    const float4 *src = reinterpret_cast<const float4 *>(a.q + s * a.q_stride + (size_t)(g.j * a.G + h) * kKvD) + l8;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        v[k] = rr < a.rows ? __ldcg(src + 8 * k) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    rr += 4;
-                    h += 4;
-                    while (h >= a.G) { h -= a.G; ++s; }
-                };
-#pragma unroll
-                for (int i = 0; i < 2; ++i) fetch(x[i]);
-                // rolled: code that runs once a piece costs its instruction fetches
+            if (g.nt == 2 || b == 0) {
+                const int sub = lane >> 3, l8 = lane & 7;          // eight lanes a row, four rows a step
+                uint8_t *qd = qbuf + (g.nt == 2 ? (size_t)b * kPreQBytes : 0) + (32 * (warp & 3) + sub) * 128;
+                const int row0 = tile0 + 32 * (warp & 3) + sub, s0 = row0 / a.G;
+                int h = row0 - s0 * a.G;
+                const float *src = a.q + s0 * a.q_stride + (size_t)(g.j * a.G + h) * kKvD + 4 * l8;
+                const int64_t wrap = a.q_stride - (int64_t)a.G * kKvD;         // to the next sequence's heads
+                uint32_t dst = smem_addr(qd + l8 * 16);
 #pragma unroll 1
-                for (int i0 = 0; i0 < 8; i0 += 2)
+                for (int i = 0; i < 8; ++i, dst += 512u) {
+                    const bool in = row0 + 4 * i < a.rows;
+                    const float *p = in ? src : a.q;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        float4 v[4];
-                        float mx = 0.f;
+                    for (int k = 0; k < 4; ++k) cp_async16(dst + 16384u * k, p + 32 * k, in);
+                    src += 4 * kKvD;
+                    for (h += 4; h >= a.G; h -= a.G) src += wrap;
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+                __syncwarp();
+#pragma unroll 2
+                for (int i = 0; i < 8; ++i) {
+                    float4 v[4];
+                    float mx = 0.f;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            v[k] = x[i][k];
-                            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
-                        }
-                        if (i0 < 6) fetch(x[i]);
-#pragma unroll
-                        for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                        const float p2 = pow2_of(mx), inv = inv_pow2(p2) * a.qsign;
-                        const float mine = __shfl_sync(0xffffffffu, p2, (lane & 3) * 8);
-                        if (lane >> 2 == i0 + i) c2 = fmaxf(a.cscale * mine, 1.17549435e-38f);   // not 0: a masked score is -inf c2
-                        const int rt = 32 * (warp & 3) + 4 * (i0 + i) + sub;                    // row of the tile
-                        if (put)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const float y[4] = {v[k].x * inv, v[k].y * inv, v[k].z * inv, v[k].w * inv};
-                                const float h4[4] = {hi_part(y[0]), hi_part(y[1]), hi_part(y[2]), hi_part(y[3])};
-                                // dims 32 k + 4 l8 ..: 16-byte granule 4 k + l8 / 2 of the row, 8 granules a block
-                                const uint32_t off = (uint32_t)(k >> 1) * 16384u + sw128_off(rt, 4 * (k & 1) + (l8 >> 1));
-                                *reinterpret_cast<uint2 *>(qd + off) =
-                                    make_uint2(pack_h2(h4[0], h4[1]), pack_h2(h4[2], h4[3]));
-                                *reinterpret_cast<uint2 *>(qd + 32768 + off) =
-                                    make_uint2(pack_h2(y[0] - h4[0], y[1] - h4[1]), pack_h2(y[2] - h4[2], y[3] - h4[3]));
-                            }
+                    for (int k = 0; k < 4; ++k) {
+                        v[k] = *reinterpret_cast<const float4 *>(qd + i * 512 + l8 * 16 + 16384 * k);   // dims 32 k + 4 l8 ..
+                        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
                     }
+#pragma unroll
+                    for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    const float p2 = pow2_of(mx), inv = inv_pow2(p2) * a.qsign;
+                    const float mine = __shfl_sync(0xffffffffu, p2, (lane & 3) * 8);    // also: the rows have been read
+                    if (lane >> 2 == i) c2 = fmaxf(a.cscale * mine, 1.17549435e-38f);   // not 0: a masked score is -inf c2
+                    const uint32_t row7 = (uint32_t)(sub + 4 * i) & 7u;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float y[4] = {v[k].x * inv, v[k].y * inv, v[k].z * inv, v[k].w * inv};
+                        const float h4[4] = {hi_part(y[0]), hi_part(y[1]), hi_part(y[2]), hi_part(y[3])};
+                        // granule 4 (k % 2) + l8 / 2 of the row of block k / 2, swizzled as the operand wants it
+                        uint8_t *to = qd + i * 512 + (k >> 1) * 16384 +
+                                      (((4u * (k & 1) + (uint32_t)(l8 >> 1)) ^ row7) << 4) + (l8 & 1) * 8;
+                        *reinterpret_cast<uint2 *>(to) = make_uint2(pack_h2(h4[0], h4[1]), pack_h2(h4[2], h4[3]));
+                        *reinterpret_cast<uint2 *>(to + 32768) =
+                            make_uint2(pack_h2(y[0] - h4[0], y[1] - h4[1]), pack_h2(y[2] - h4[2], y[3] - h4[3]));
+                    }
+                }
+                if (g.nt == 1) c_of[r] = c2;                       // for buffer 1, which has the same rows
             }
             fence_proxy_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
-            float m = -INFINITY, l = 0.f;
             bool ok = true;
+            if (g.nt == 1 && b == 1) {
+                ok = __all_sync(0xffffffffu, wait_or_abort(q_full, pq, abort_flag));
+                c2 = c_of[r];
+            }
+            pq ^= 1u;
+            float m = -INFINITY, l = 0.f;
             int unit = 0;
             // this buffer's token tiles: every one (nt 2), or every second one
             const int first = g.nt == 2 ? 0 : b, step = g.nt == 2 ? 1 : 2;
-            for (int i = first; i < n; i += step, ++unit) {
+            for (int i = first; ok && i < n; i += step, ++unit) {
                 ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[b], ps, abort_flag));
                 if (!ok) break;
                 ps ^= 1u;
