@@ -4,6 +4,8 @@
 #pragma once
 #include "li_common.cuh"
 
+#include <atomic>
+
 namespace li {
 
 constexpr int kKvD = 128;              // head_dim of the cache (the only built size)
@@ -23,6 +25,20 @@ inline int check_kv_cache(const li_kv_cache *C) {
     // (sequence, kv head, slot) counts stay below 2^40, (sequence, kv head) pairs below 2^31
     if ((int64_t)C->n_seqs * C->n_kv_heads >= (1ll << 31)) return LI_ERR_BAD_SHAPE;
     return 0;
+}
+
+// Lets a kernel take `smem` bytes of dynamic shared memory on the current
+// device, once per device (bit d of `done`: set on device d).
+template <typename Kernel>
+int allow_smem(Kernel kernel, size_t smem, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+    if (done.load(std::memory_order_relaxed) & bit) return 0;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return (int)e;
 }
 
 // li_rope as the kernels read it: the frequency of pair i in turns per

@@ -91,6 +91,8 @@ struct KvAttnArgs {
     float *score;                      // [B][Hq][score_stride], log2 units (weight != nullptr)
     int score_stride;                  // max_ctx rounded up to 4
     bool after_prefix;
+    int lead;                          // prefix tokens that kv_own takes as every sequence's first (else 0)
+    const __half *kp, *vp;
     // prefix part
     int n_prefix, rows, n_rt, per_group, n_grp, n_tt;   // rows = B G; row tiles; row tiles per group; groups; tiles
     int pre_ctas, slots;
@@ -110,6 +112,9 @@ __device__ __forceinline__ int own_len(const KvAttnArgs &a, int s) {
     const int n = __ldcg(a.len + s);
     return n < 0 || n > a.max_ctx ? 0 : n;
 }
+
+// Tokens of sequence s that kv_own works on.
+__device__ __forceinline__ int own_tokens(const KvAttnArgs &a, int s) { return own_len(a, s) + a.lead; }
 
 __device__ __forceinline__ int own_steps(int n) { return (n + kOwnTok - 1) / kOwnTok; }
 
@@ -180,7 +185,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 
 // NG groups of 8 q heads. In a warp, lane l holds q head l / 4 of each group
 // (scores of tokens 2 (l % 4), +1 of each 8; dims 2 (l % 4), +1 of each 8).
-template <int NG, bool SCORE>
+template <int NG, bool SCORE, bool LEAD>
 __global__ void __launch_bounds__(kOwnThreads, 1) kv_own_kernel(const __grid_constant__ KvAttnArgs a) {
     extern __shared__ __align__(128) uint8_t own_smem[];
     __shared__ int cum[kScanMax], wsum[kOwnWarps];
@@ -201,11 +206,9 @@ __global__ void __launch_bounds__(kOwnThreads, 1) kv_own_kernel(const __grid_con
             const int s = e * per + i;
             if (e < entries && s < a.B) {
                 const int n = __ldcg(a.len + s);
-                if (n < 0 || n > a.max_ctx) {
-                    if (blockIdx.x == 0) atomicExch(&g_device_error, LI_ERR_BAD_ARG);
-                } else {
-                    mine += own_steps(n);
-                }
+                const bool bad = n < 0 || n > a.max_ctx;
+                if (bad && blockIdx.x == 0) atomicExch(&g_device_error, LI_ERR_BAD_ARG);
+                mine += own_steps((bad ? 0 : n) + a.lead);
             }
         }
         mine *= a.Hkv;
@@ -230,7 +233,7 @@ __global__ void __launch_bounds__(kOwnThreads, 1) kv_own_kernel(const __grid_con
                 int at = off + incl - mine;
                 for (int i = 0; i < per && e * per + i < a.B; ++i) {
                     a.base[e * per + i] = at;
-                    at += own_steps(own_len(a, e * per + i)) * a.Hkv;
+                    at += own_steps(own_tokens(a, e * per + i)) * a.Hkv;
                 }
             }
         }
@@ -254,10 +257,10 @@ __global__ void __launch_bounds__(kOwnThreads, 1) kv_own_kernel(const __grid_con
                 const int mid = (e + end) / 2;
                 if (cum[mid] <= lo) e = mid; else end = mid;
             }
-            int at = cum[e], s = e * per, n = own_len(a, s);
+            int at = cum[e], s = e * per, n = own_tokens(a, s);
             while (at + own_steps(n) * a.Hkv <= lo) {
                 at += own_steps(n) * a.Hkv;
-                n = own_len(a, ++s);
+                n = own_tokens(a, ++s);
             }
             const int in = lo - at, st = own_steps(n);
             ld.s = s; ld.n = n; ld.j = in / st; ld.t = in - ld.j * st;
@@ -269,7 +272,7 @@ __global__ void __launch_bounds__(kOwnThreads, 1) kv_own_kernel(const __grid_con
             c.j = 0;
             do {
                 if (++c.s >= a.B) { c.n = 0; return; }
-                c.n = own_len(a, c.s);
+                c.n = own_tokens(a, c.s);
             } while (c.n == 0);
         };
         Cursor cu = ld;
@@ -277,17 +280,26 @@ __global__ void __launch_bounds__(kOwnThreads, 1) kv_own_kernel(const __grid_con
         const size_t row = (size_t)a.Hkv * kKvD;
         const int lr = lane >> 4, lc = lane & 15;      // this lane's row (of two) and 16-byte piece in a copy
         auto issue = [&](const Cursor &c, int stage) {
-            const size_t at = ((size_t)c.s * a.max_ctx + (size_t)c.t * kOwnTok) * row + (size_t)c.j * kKvD + 8 * lc;
-            const int left = c.n - c.t * kOwnTok;
+            const int t0 = c.t * kOwnTok, left = c.n - t0;
+            const size_t col = (size_t)c.j * kKvD + 8 * lc, seq = (size_t)c.s * a.max_ctx;
+            const size_t at = (seq + t0) * row + col;
             const uint32_t dst = ring + (uint32_t)stage * kOwnStageBytes;
 #pragma unroll
             for (int i = 0; i < kOwnTok / 2; ++i) {
                 const int r = 2 * i + lr;
                 const bool ok = r < left;              // past the length: zeros, whatever the slot holds
-                const size_t src = at + (ok ? (size_t)r * row : 0);
                 const uint32_t d = dst + (uint32_t)(r * 256 + ((lc ^ (r & 7)) << 4));
-                cp_async16(d, a.k + src, ok);
-                cp_async16(d + kOwnTok * 256, a.v + src, ok);
+                if (LEAD) {                            // the prefix, then the sequence's slots
+                    const int t = t0 + (ok ? r : 0);
+                    const bool pre = t < a.lead;
+                    const size_t src = (pre ? (size_t)t : seq + (t - a.lead)) * row + col;
+                    cp_async16(d, (pre ? a.kp : a.k) + src, ok);
+                    cp_async16(d + kOwnTok * 256, (pre ? a.vp : a.v) + src, ok);
+                } else {
+                    const size_t src = at + (ok ? (size_t)r * row : 0);
+                    cp_async16(d, a.k + src, ok);
+                    cp_async16(d + kOwnTok * 256, a.v + src, ok);
+                }
             }
         };
 #pragma unroll
@@ -378,8 +390,9 @@ __global__ void __launch_bounds__(kOwnThreads, 1) kv_own_kernel(const __grid_con
                 for (int x = 0; x < 4; ++x) {
                     const int nt = x >> 1, r = x & 1, tok = 8 * nt + 2 * tq + r;
                     s2[x] = (sc[e][nt][r] + sc[e][nt][2 + r]) * c2[e];
-                    if (SCORE && 8 * e + g < a.G && tok < left)
-                        a.score[((size_t)cu.s * a.Hq + (size_t)cu.j * a.G + 8 * e + g) * a.score_stride + t0 + tok] = s2[x];
+                    if (SCORE && 8 * e + g < a.G && tok < left && (!LEAD || t0 + tok >= a.lead))
+                        a.score[((size_t)cu.s * a.Hq + (size_t)cu.j * a.G + 8 * e + g) * a.score_stride + t0 + tok -
+                                (LEAD ? a.lead : 0)] = s2[x];
                     if (tok >= left) s2[x] = -INFINITY;
                     mx = fmaxf(mx, s2[x]);
                 }
@@ -1018,7 +1031,7 @@ __device__ __forceinline__ RowPieces pieces_of(const KvAttnArgs &a, int j, int r
     const int s = row / a.G;
     x.gq = row - s * a.G;
     x.n_pre = x.n_own = 0;
-    const int n = own_len(a, s), T = __ldcg(a.base + a.B), b0 = __ldcg(a.base + s);
+    const int n = own_tokens(a, s), T = __ldcg(a.base + a.B), b0 = __ldcg(a.base + s);
     if (a.n_prefix > 0) {
         const int rt = row / kPreRows;
         x.prow = row - rt * kPreRows;
@@ -1186,16 +1199,17 @@ __global__ void __launch_bounds__(kJoinWarps * kWarp, 3) kv_join_kernel(const __
     const float *sc = a.score + ((size_t)s * a.Hq + (size_t)j * a.G) * a.score_stride;
     const bool vec = (a.max_ctx & 3) == 0 && ((uintptr_t)a.weight & 15u) == 0;
     for (int t = chunk * kJoinRun + 4 * tid; t < n; t += a.w_chunks * kJoinRun) {
-        float w[4] = {0.f, 0.f, 0.f, 0.f};
+        // the step's probabilities are summed first: one rounding against the accumulated weight
+        float w[4] = {0.f, 0.f, 0.f, 0.f}, old[4] = {0.f, 0.f, 0.f, 0.f};
         const bool whole = vec && t + 4 <= n;
         if (a.decay != 0.f) {
             if (whole) {
                 const float4 v = *reinterpret_cast<const float4 *>(wt + t);
-                w[0] = a.decay * v.x; w[1] = a.decay * v.y; w[2] = a.decay * v.z; w[3] = a.decay * v.w;
+                old[0] = v.x; old[1] = v.y; old[2] = v.z; old[3] = v.w;
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (t + e < n) w[e] = a.decay * wt[t + e];
+                    if (t + e < n) old[e] = wt[t + e];
             }
         }
         // a row of scores has score_stride floats, a multiple of 4: past n it holds nothing, and none of it is kept
@@ -1208,6 +1222,8 @@ __global__ void __launch_bounds__(kJoinWarps * kWarp, 3) kv_join_kernel(const __
             w[2] = fmaf(ex2(v.z - m), inv, w[2]);
             w[3] = fmaf(ex2(v.w - m), inv, w[3]);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = fmaf(a.decay, old[e], w[e]);
         if (whole) {
             *reinterpret_cast<float4 *>(wt + t) = make_float4(w[0], w[1], w[2], w[3]);
         } else {
@@ -1262,7 +1278,14 @@ size_t plan(const li_kv_cache *C, int n_q_heads, KvAttnArgs *a, size_t *off /* [
     const int sms = num_sms();
     a->B = C->n_seqs; a->Hq = n_q_heads; a->Hkv = C->n_kv_heads; a->G = n_q_heads / C->n_kv_heads;
     a->max_ctx = C->max_ctx; a->n_prefix = C->n_prefix;
-    const int64_t pairs = (int64_t)a->B * a->Hkv, most = pairs * ((a->max_ctx + kOwnTok - 1ll) / kOwnTok);
+    const int64_t pairs = (int64_t)a->B * a->Hkv;
+    // A prefix that is little to read even once per sequence (30 MB: about 5 us), or that has one reader, goes with
+    // the own tokens: one kernel less, and no tile of 128 rows for a few.
+    if (a->n_prefix > 0 && (a->B == 1 || pairs * a->n_prefix * (4ll * kKvD) <= (30ll << 20))) {
+        a->lead = a->n_prefix;
+        a->n_prefix = 0;
+    }
+    const int64_t most = pairs * ((a->max_ctx + (int64_t)a->lead + kOwnTok - 1) / kOwnTok);
     if (most >= (1ll << 30) || pairs * a->G >= (1ll << 30)) return 0;
     int64_t grid = most / kOwnMinSteps;
     grid = grid < 1 ? 1 : grid < sms ? grid : sms;
@@ -1293,13 +1316,17 @@ size_t plan(const li_kv_cache *C, int n_q_heads, KvAttnArgs *a, size_t *off /* [
     return at;
 }
 
+template <int NG, bool SCORE, bool LEAD>
+int launch_own(const KvAttnArgs &a, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    if (const int rc = allow_smem(kv_own_kernel<NG, SCORE, LEAD>, kOwnSmem, done)) return rc;
+    return (int)launch_pdl(kv_own_kernel<NG, SCORE, LEAD>, dim3((unsigned)(a.own_warps / kOwnWarps)),
+                           dim3(kOwnThreads), kOwnSmem, s, true, a);
+}
+
 template <int NG, bool SCORE>
 int launch_own(const KvAttnArgs &a, cudaStream_t s) {
-    const cudaError_t e = cudaFuncSetAttribute(kv_own_kernel<NG, SCORE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)kOwnSmem);
-    if (e != cudaSuccess) return (int)e;
-    return (int)launch_pdl(kv_own_kernel<NG, SCORE>, dim3((unsigned)(a.own_warps / kOwnWarps)), dim3(kOwnThreads),
-                           kOwnSmem, s, true, a);
+    return a.lead ? launch_own<NG, SCORE, true>(a, s) : launch_own<NG, SCORE, false>(a, s);
 }
 
 }  // namespace
@@ -1344,6 +1371,7 @@ int li::attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_stride, i
     char *ws = static_cast<char *>(workspace);
     a.q = q; a.q_stride = q_stride;
     a.k = static_cast<const __half *>(C->k); a.v = static_cast<const __half *>(C->v);
+    a.kp = static_cast<const __half *>(C->k_prefix); a.vp = static_cast<const __half *>(C->v_prefix);
     a.len = C->len;
     a.cscale = fabsf(scale) * kLog2e; a.qsign = scale < 0.f ? -1.f : 1.f;
     a.decay = decay; a.out = out; a.weight = C->weight;
@@ -1363,9 +1391,8 @@ int li::attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_stride, i
         if ((rc = encode_prefix(&mk, C->k_prefix, a.Hkv, a.n_prefix)) ||
             (rc = encode_prefix(&mv, C->v_prefix, a.Hkv, a.n_prefix)))
             return rc;
-        const cudaError_t e = cudaFuncSetAttribute(kv_prefix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (int)kPreSmem);
-        if (e != cudaSuccess) return (int)e;
+        static std::atomic<uint64_t> done{0};
+        if ((rc = allow_smem(kv_prefix_kernel, kPreSmem, done))) return rc;
         if ((rc = (int)launch_pdl(kv_prefix_kernel, dim3((unsigned)a.pre_ctas), dim3(kPreThreads), kPreSmem, st, true,
                                   mk, mv, a)))
             return rc;
@@ -1376,7 +1403,7 @@ int li::attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_stride, i
     // warps per 4 rows: as many as it takes to fill the SMs, up to the pieces that a row can have
     const int pairs = a.B * a.Hkv;
     const int64_t pre = a.n_prefix ? 2ll * a.pre_ctas / (a.Hkv * a.n_grp) + 2 : 0;
-    int64_t own = (a.max_ctx + kOwnTok - 1) / kOwnTok / kOwnMinSteps + 1;
+    int64_t own = (a.max_ctx + (int64_t)a.lead + kOwnTok - 1) / kOwnTok / kOwnMinSteps + 1;
     if (own > a.own_warps / pairs + 2) own = a.own_warps / pairs + 2;
     const int64_t row_blocks = (int64_t)a.Hkv * ((a.B * a.G + kJoinRows - 1) / kJoinRows);
     a.wpr = 1;

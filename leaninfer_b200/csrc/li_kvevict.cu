@@ -273,12 +273,8 @@ size_t al256(size_t v) { return (v + 255) / 256 * 256; }
 
 template <int THREADS>
 int launch_select(const EvictArgs &a, bool cached, size_t smem, cudaStream_t s) {
-    if (smem > 32 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kv_select_kernel<THREADS>,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (kSelCacheMax + kSelCacheMax / 32) * 4);
-        if (e != cudaSuccess) return (int)e;
-    }
+    static std::atomic<uint64_t> done{0};
+    if (const int rc = allow_smem(kv_select_kernel<THREADS>, (kSelCacheMax + kSelCacheMax / 32) * 4, done)) return rc;
     return (int)launch_pdl(kv_select_kernel<THREADS>, dim3((unsigned)a.n_pairs), dim3(THREADS), smem, s, true, a, cached);
 }
 

@@ -355,9 +355,63 @@ def test_attention_variants(cuda, kw):
     _attn_check(cuda, rng(600), 7, 333, 200, [200, 0, 1, 64, 100, 199, 16], 2, 5, **kw)
 
 
+# Prefixes beyond the size that goes with the own tokens (30 MB, read once per
+# sequence): the tensor-core kernel.
+PREFIX = [
+    # B, P, ctx, lens, Hkv, G
+    (2, 40000, 40, [40, 7], 1, 8),                            # 16 rows: one row tile, alternate token tiles
+    (9, 8200, 50, list(range(9)), 1, 16),                     # 144 rows: two row tiles
+    (26, 2500, 20, [20] * 26, 1, 5),                          # 130 rows, the second tile nearly empty
+    (70, 1000, 40, [i % 41 for i in range(70)], 1, 5),        # 350 rows: three row tiles
+    (70, 7001, 9, [i % 10 for i in range(70)], 2, 5),         # three, in a pair and a single
+    (130, 300, 9, [i % 10 for i in range(130)], 2, 4),        # 520 rows: five
+    (620, 100, 3, [i % 4 for i in range(620)], 1, 1),         # five row tiles of one token tile each
+    (300, 128, 40, [i % 41 for i in range(300)], 2, 3),       # one whole token tile
+    (40, 769, 1, [i % 2 for i in range(40)], 2, 7),
+    (64, 4096, 2, [0] * 64, 1, 6),                            # no own tokens
+]
+
+
+@pytest.mark.parametrize("case", range(len(PREFIX)))
+def test_attention_over_a_large_prefix(cuda, case):
+    B, P, ctx, lens, Hkv, G = PREFIX[case]
+    assert B > 1 and B * Hkv * P * 512 > 30 << 20
+    _attn_check(cuda, rng(560 + case), B, P, ctx, lens, Hkv, G, decay=[1.0, 0.0, 0.75][case % 3])
+
+
+@pytest.mark.parametrize("kw", [
+    dict(weight=False), dict(gap=20), dict(q_scale=1e6, scale=1e-7), dict(q_scale=1e-20), dict(q_scale=0.0),
+    dict(q_scale=40.0), dict(k_scale=1000.0, scale=1e-4), dict(scale=0.0), dict(scale=-0.3), dict(graph=True),
+    dict(graph=True, weight=False)])
+def test_large_prefix_variants(cuda, kw):
+    """The variants above on the tensor-core kernel."""
+    _attn_check(cuda, rng(600), 20, 1700, 70, [(i * 13) % 71 for i in range(20)], 2, 5, **kw)
+
+
+def test_large_prefix_growing_scores(cuda):
+    """Scores that rise along the prefix by far more than the lag of the
+    running maximum, and fall, and jump: every rescaling path."""
+    import torch
+    from leaninfer_b200 import ops
+    from oracle import kv
+    r = rng(630)
+    B, P, Hkv, G = 24, 3000, 1, 4
+    c, t, cache = _cache(r, cuda, B, 8, Hkv, [8] * B, P, weight=False)
+    ramp = np.concatenate([np.linspace(-3, 3, 1500), np.linspace(3, -3, 1200), np.full(299, -2.0), [6.0]])
+    c["kp"] = (0.05 * c["kp"].astype(np.float32) + ramp[:, None, None]).astype(np.float16)
+    t["kp"].copy_(T(c["kp"], cuda))
+    q = (r.standard_normal((B, G, 128)) * 0.2 + r.choice([-0.3, 0.3, 0.05], (B, G, 1))).astype(np.float32)
+    got = cache.decode(T(q, cuda)).double().cpu().numpy()
+    ref, _ = kv.attn(q, c["k"], c["v"], c["lens"], c["kp"], c["vp"])
+    S = float(np.abs(q).astype(np.float64).sum(-1).max() * np.abs(c["kp"].astype(np.float64)).max()) * 128 ** -0.5
+    assert np.abs(got - ref).max() <= (2.0 ** -16 * S + 2.0 ** -17) * 5
+    assert ops.device_status() == 0
+
+
 def test_attention_bad_lengths(cuda):
     """Lengths outside the cache count as no own slots and raise the flag."""
     _attn_check(cuda, rng(610), 4, 70, 20, [21, -1, 20, 2**31 - 1], 2, 3)
+    _attn_check(cuda, rng(611), 20, 1700, 20, [21, -1, 20, 2**31 - 1] * 5, 2, 3)
 
 
 def test_attention_is_deterministic_and_stream_ordered(cuda):
@@ -365,7 +419,7 @@ def test_attention_is_deterministic_and_stream_ordered(cuda):
     import torch
     r = rng(620)
     sets = []
-    for P in (700, 0):
+    for P in (2000, 100):
         c, t, cache = _cache(r, cuda, 20, 500, 2, list(range(0, 500, 25)), P)
         q = T(r.standard_normal((20, 10, 128)).astype(np.float32), cuda)
         sets.append((cache, q, cache.decode(q, decay=0.0), t["weight"]))
