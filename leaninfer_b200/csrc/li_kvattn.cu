@@ -1041,7 +1041,8 @@ __device__ __forceinline__ RowPieces pieces_of(const KvAttnArgs &a, int j, int r
         x.len = runs.len; x.extra = runs.extra; x.base = g.base; x.nt = g.nt;
         x.c0 = runs.taker(g.base);
         const int c1 = runs.taker(g.base + g.nt * a.n_tt - 1);
-        x.streams = g.nt == 2 ? 1 : 2;
+        // one record per buffer; runs of one tile leave buffer 1 none
+        x.streams = g.nt == 2 || runs.len + (runs.extra ? 1 : 0) <= 1 ? 1 : 2;
         x.stream0 = g.nt == 2 ? rt - g.rt : 0;
         x.n_pre = (c1 - x.c0 + 1) * x.streams;
     }
