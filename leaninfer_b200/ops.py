@@ -349,32 +349,32 @@ _ROPE_LAYOUTS = {"interleaved": LI_ROPE_INTERLEAVED, "half": LI_ROPE_HALF}
 def _on(index: int, *tensors) -> None:
     """The tensors lie on cuda:index, and it is the current device (the
     library launches on the current device's stream)."""
-    for t in tensors:
-        if t is not None and t.get_device() != index:
-            raise ValueError("LeanInfer kernels take CUDA tensors of one device")
     if index < 0:
         raise ValueError("LeanInfer kernels take CUDA tensors")
     if index != torch.cuda.current_device():
         raise ValueError(f"tensors on cuda:{index}, but cuda:{torch.cuda.current_device()} is the current device")
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValueError("LeanInfer kernels take CUDA tensors of one device")
 
 
-def _heads(t: torch.Tensor, n: int, heads: int | None, dim: int, dtype, what: str) -> int:
+def _heads(t: torch.Tensor, n: int, heads: int, dim: int, dtype, what: str) -> int:
     """Checks [n, heads, dim] with each token's heads contiguous and any token
     stride; returns that stride."""
-    shape, st = t.shape, t.stride()
-    if len(shape) != 3 or shape[0] != n or shape[2] != dim or (heads is not None and shape[1] != heads):
-        raise ValueError(f"{what}: expected [{n}, {heads or 'heads'}, {dim}], got {tuple(shape)}")
-    if st[2] != 1 or (st[1] != dim and shape[1] > 1):
+    if t.shape != (n, heads, dim):
+        raise ValueError(f"{what}: expected [{n}, {heads}, {dim}], got {tuple(t.shape)}")
+    token, head, one = t.stride()
+    if one != 1 or (head != dim and heads > 1):
         raise ValueError(f"{what}: the heads of a token must be contiguous")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{what}: expected {dtype}, got {t.dtype}")
-    return st[0]
+    return token
 
 
 def _index(t: torch.Tensor | None, n: int, what: str) -> int | None:
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous int32 tensor of {n} values")
     return t.data_ptr()
 
@@ -477,6 +477,8 @@ class KVCache:
         qp = op = None
         qs = os = hq = 0
         if q is not None:
+            if q.dim() != 3:
+                raise ValueError(f"q: expected [{n}, heads, {dim}]")
             hq = q.shape[1]
             qs = _heads(q, n, hq, dim, dt, "q")
             if q_out is None:
@@ -493,8 +495,10 @@ class KVCache:
         """Attention of q [n_seqs, n_q_heads, 128] (fp32) over the prefix and
         each sequence's first len slots; returns [n_seqs, n_q_heads, 128]. With
         weight in the cache, weight = decay * weight + this step's."""
-        qs = _heads(q, self.n_seqs, None, self.head_dim, torch.float32, "q")
+        if q.dim() != 3:
+            raise ValueError(f"q: expected [{self.n_seqs}, heads, {self.head_dim}]")
         hq = q.shape[1]
+        qs = _heads(q, self.n_seqs, hq, self.head_dim, torch.float32, "q")
         if out is None:
             out = torch.empty(self.n_seqs, hq, self.head_dim, device=self.device, dtype=torch.float32)
         elif out.shape != q.shape or not out.is_contiguous() or out.dtype != torch.float32:
