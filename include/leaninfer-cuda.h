@@ -482,8 +482,9 @@ int li_launch_kv_append(const li_kv_cache * C, const li_rope * R, int dtype,
  * its softmax probability (decay 1: accumulated, 0: replaced); slots past
  * len[s] are left alone. A length outside 0 .. max_ctx is taken as 0 own
  * slots and li_device_status() reports LI_ERR_BAD_ARG. Hq / Hkv in 1 .. 16;
- * q, out 16-byte aligned, q_stride a multiple of 4. No counterpart among the
- * reference's kernels. */
+ * scale and decay finite, decay >= 0; q, out 16-byte aligned, q_stride a
+ * multiple of 4; out may be q where the layouts agree. No counterpart among
+ * the reference's kernels. */
 size_t li_attn_kv_workspace_size(const li_kv_cache * C, int n_q_heads);
 int li_launch_attn_kv_decode(const li_kv_cache * C, const float * q, int64_t q_stride, int n_q_heads,
         float scale, float * out, float decay, void * workspace, size_t workspace_bytes, void * stream);

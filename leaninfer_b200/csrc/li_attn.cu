@@ -1051,7 +1051,7 @@ extern "C" int li_launch_attn_layer_decode_kv(const li_attn_layer *L, const li_r
                                               const float *x, float *y, const int32_t *pos, float decay,
                                               void *workspace, size_t workspace_bytes, void *stream) {
     if (const int rc = check_layer_kv(L, C)) return rc;
-    if (!x || !y || !pos || !(decay >= 0.0f)) return LI_ERR_BAD_ARG;
+    if (!x || !y || !pos || !(decay >= 0.0f) || isinf(decay)) return LI_ERR_BAD_ARG;
     KvPrepArgs a = {};
     li_rope from_layer = {};
     if (!R) {

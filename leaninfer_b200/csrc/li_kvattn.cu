@@ -1287,7 +1287,7 @@ size_t plan(const li_kv_cache *C, int n_q_heads, KvAttnArgs *a, size_t *off /* [
         a->n_prefix = 0;
     }
     const int64_t most = pairs * ((a->max_ctx + (int64_t)a->lead + kOwnTok - 1) / kOwnTok);
-    if (most >= (1ll << 30) || pairs * a->G >= (1ll << 30)) return 0;
+    if (most >= (1ll << 30) || pairs * a->G >= (1ll << 30) || a->max_ctx + (int64_t)a->lead >= (1ll << 30)) return 0;
     int64_t grid = most / kOwnMinSteps;
     grid = grid < 1 ? 1 : grid < sms ? grid : sms;
     a->own_warps = (int)grid * kOwnWarps;
@@ -1357,7 +1357,7 @@ int li::attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_stride, i
                        float decay, const float *gate, int64_t gate_stride, void *workspace, size_t workspace_bytes,
                        void *stream) {
     if (const int rc = check_kv_cache(C)) return rc;
-    if (!q || !out || n_q_heads <= 0 || !(decay >= 0.0f)) return LI_ERR_BAD_ARG;
+    if (!q || !out || n_q_heads <= 0 || !(decay >= 0.0f) || isinf(decay) || !isfinite(scale)) return LI_ERR_BAD_ARG;
     if (n_q_heads % C->n_kv_heads) return LI_ERR_BAD_SHAPE;
     if (n_q_heads / C->n_kv_heads > 16) return LI_ERR_UNSUPPORTED;
     if (!aligned16(q) || !aligned16(out) || q_stride % 4) return LI_ERR_MISALIGNED;

@@ -417,6 +417,8 @@ def rope(rope: Rope, x: torch.Tensor, pos: torch.Tensor, out: torch.Tensor | Non
     if out.dtype != x.dtype:
         raise ValueError(f"out: expected {x.dtype}, got {out.dtype}")
     _on(x.get_device(), out, pos, rope.keep)
+    if x.numel() == 0:
+        return out
     xs, os = x.stride(), out.stride()
     check(_lib.load().li_launch_rope(rope.ref, _DTYPES[x.dtype], x.data_ptr(), out.data_ptr(), _index(pos, n, "pos"),
                                      n, heads, xs[0], xs[1], os[0], os[1], transpose, _stream()), "li_launch_rope")
@@ -485,6 +487,8 @@ class KVCache:
                 q_out = torch.empty(n, hq, dim, device=self.device, dtype=dt)
             os = _heads(q_out, n, hq, dim, dt, "q_out")
             qp, op = q.data_ptr(), q_out.data_ptr()
+        if n == 0:
+            return q_out if q is not None else None
         check(_lib.load().li_launch_kv_append(
             self.ref, rope.ref if rope is not None else None, _DTYPES[dt], qp, qs, op, os, hq, k.data_ptr(), ks,
             v.data_ptr(), vs, _index(pos, n, "pos"), _index(seq, n, "seq"), _index(slot, n, "slot"), n, _stream()),
@@ -504,6 +508,8 @@ class KVCache:
         elif out.shape != q.shape or not out.is_contiguous() or out.dtype != torch.float32:
             raise ValueError("out: expected a contiguous fp32 tensor of q's shape")
         _on(self.index, q, out, workspace)
+        if self.n_seqs == 0:
+            return out
         lib = _lib.load()
         ws = workspace if workspace is not None else self._workspace(
             hq, lambda: int(lib.li_attn_kv_workspace_size(self.ref, hq)))
@@ -517,6 +523,8 @@ class KVCache:
         li_launch_kv_evict); pos int32 [n_seqs], the newest token's position;
         n_sink counts own tokens, after the prefix."""
         _on(self.index, pos, workspace)
+        if self.n_seqs == 0:
+            return
         lib = _lib.load()
         ws = workspace if workspace is not None else self._workspace(
             ("evict", budget), lambda: int(lib.li_kv_evict_workspace_size(self.ref, budget)))

@@ -414,6 +414,44 @@ def test_attention_bad_lengths(cuda):
     _attn_check(cuda, rng(611), 20, 1700, 20, [21, -1, 20, 2**31 - 1] * 5, 2, 3)
 
 
+def test_empty_calls(cuda):
+    """No tokens, no sequences: nothing happens."""
+    import torch
+    from leaninfer_b200 import ops
+    R = ops.Rope(head_dim=128, rope_dim=64)
+    none = torch.empty(0, device=cuda, dtype=torch.int32)
+    assert ops.rope(R, torch.empty(0, 3, 128, device=cuda), none).shape == (0, 3, 128)
+    k = torch.zeros(2, 4, 2, 128, device=cuda, dtype=torch.float16)
+    cache = ops.KVCache(k, k.clone(), torch.ones(2, device=cuda, dtype=torch.int32))
+    z = torch.empty(0, 2, 128, device=cuda)
+    assert cache.append(z, z, none) is None and cache.append(z, z, none, q=z).shape == (0, 2, 128)
+    k0 = k[:0]
+    cache = ops.KVCache(k0, k0.clone(), none, weight=torch.empty(0, 2, 4, device=cuda),
+                        slot_pos=torch.empty(0, 2, 4, device=cuda, dtype=torch.int32))
+    assert cache.decode(torch.empty(0, 4, 128, device=cuda)).shape == (0, 4, 128)
+    cache.evict(none, 2)
+    assert ops.device_status() == 0
+
+
+def test_output_over_the_queries(cuda):
+    """decode with out = q, and many sequences (more than the length scan's
+    entries) of very different lengths."""
+    from leaninfer_b200 import ops
+    from oracle import kv
+    r = rng(640)
+    B, ctx = 4500, 5
+    lens = r.integers(0, ctx + 1, B).astype(np.int32)
+    lens[1000:3500] = 0
+    c, t, cache = _cache(r, cuda, B, ctx, 1, lens, 0, weight=True)
+    q = r.standard_normal((B, 2, 128)).astype(np.float32)
+    qd = T(q, cuda)
+    assert cache.decode(qd, out=qd) is qd
+    ref, w_ref = kv.attn(q, c["k"], c["v"], lens, weight=c["weight"])
+    assert np.linalg.norm(qd.double().cpu().numpy() - ref) <= 1e-5 * np.linalg.norm(ref)
+    assert np.abs(t["weight"].double().cpu().numpy() - w_ref).max() <= 1e-5
+    assert ops.device_status() == 0
+
+
 def test_attention_is_deterministic_and_stream_ordered(cuda):
     """Two caches decoded in turn on two streams, twice: the same bits."""
     import torch
@@ -479,6 +517,8 @@ EVICT = [
     (2, 3000, 2, [3000, 2900], 31, 1, 30),
     (2, 300, 2, [300, 200], 300, 0, 0),
     (1, 60000, 1, [59999], 30011, 4, 1000),             # more slots than the keys' shared memory holds
+    (1, 49152, 1, [49152], 40000, 4, 100),              # as many as it holds
+    (1, 9000, 2, [9000], 3000, 4, 2900),                # more moves than the selecting block makes itself
     (5, 37, 2, [37, 38, -1, 36, 2**31 - 1], 20, 2, 3),  # lengths outside the cache
 ]
 

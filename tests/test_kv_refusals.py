@@ -130,7 +130,8 @@ def test_decode_arguments(lib):
         return lib.li_launch_attn_kv_decode(*{**ok, **kw}.values(), None)
 
     assert call(q=None) == BAD_ARG and call(out=None) == BAD_ARG and call(hq=0) == BAD_ARG
-    assert call(decay=-0.5) == BAD_ARG and call(decay=float("nan")) == BAD_ARG
+    assert call(decay=-0.5) == BAD_ARG and call(decay=float("nan")) == BAD_ARG and call(decay=float("inf")) == BAD_ARG
+    assert call(scale=float("nan")) == BAD_ARG and call(scale=float("-inf")) == BAD_ARG
     assert call(hq=7) == BAD_SHAPE and call(hq=34) == UNSUPPORTED
     assert call(q=P + 4) == MISALIGNED and call(out=P + 8) == MISALIGNED and call(qs=1023) == MISALIGNED
     assert call(ws=None) == WORKSPACE and call(wb=need - 1) == WORKSPACE and call(ws=P + 8) == MISALIGNED
@@ -210,7 +211,7 @@ def test_layer_on_a_managed_cache_arguments(lib):
                          (dict(rope_theta=0.5), BAD_ARG), (dict(in_norm_w=P + 4), MISALIGNED)):
         assert call(L=_layer(**change)) == want, change
     assert call(x=None) == BAD_ARG and call(y=None) == BAD_ARG and call(pos=None) == BAD_ARG
-    assert call(decay=-1.0) == BAD_ARG
+    assert call(decay=-1.0) == BAD_ARG and call(decay=float("inf")) == BAD_ARG
     assert call(R=_rope(head_dim=64)) == BAD_SHAPE and call(R=_rope(theta=0.0)) == BAD_ARG
     assert call(x=P + 4) == MISALIGNED and call(pos=P + 2) == MISALIGNED and call(ws=P + 8) == MISALIGNED
     assert call(ws=None) == WORKSPACE and call(wb=need - 1) == WORKSPACE
