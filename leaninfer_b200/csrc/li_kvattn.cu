@@ -839,23 +839,24 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             tiles_of(a, g.base, g.nt, lo, hi, t0, t1);
             const int n = t1 - t0;
             if (n <= 0) continue;
-            // This warp's 32 rows of q, scaled and split into the operand's rows. They are copied as they are
-            // first, all in flight at once: row r's 512 bytes are the 128-byte rows r of the operand's four blocks
-            // (hi and lo, 64 dims each), so that each row is then converted in its own place. One row tile: buffer
-            // 0's warps do it for both.
+            // This warp's rows of q (32 of its buffer's tile, or 16 of the one tile), scaled and split into the
+            // operand's rows. They are copied as they are first, all in flight at once: row r's 512 bytes are the
+            // 128-byte rows r of the operand's four blocks (hi and lo, 64 dims each), so that each row is then
+            // converted in its own place.
             const int tile0 = (g.rt + (g.nt == 2 ? b : 0)) * kPreRows, row = tile0 + r;
             const bool live = row < a.rows;
             float c2 = 0.f;
-            if (g.nt == 2 || b == 0) {
+            {
                 const int sub = lane >> 3, l8 = lane & 7;          // eight lanes a row, four rows a step
-                uint8_t *qd = qbuf + (g.nt == 2 ? (size_t)b * kPreQBytes : 0) + (32 * (warp & 3) + sub) * 128;
-                const int row0 = tile0 + 32 * (warp & 3) + sub, s0 = row0 / a.G;
+                const int steps = g.nt == 2 ? 8 : 4, first_row = g.nt == 2 ? 32 * (warp & 3) : 16 * warp;
+                uint8_t *qd = qbuf + (g.nt == 2 ? (size_t)b * kPreQBytes : 0) + (first_row + sub) * 128;
+                const int row0 = tile0 + first_row + sub, s0 = row0 / a.G;
                 int h = row0 - s0 * a.G;
                 const float *src = a.q + s0 * a.q_stride + (size_t)(g.j * a.G + h) * kKvD + 4 * l8;
                 const int64_t wrap = a.q_stride - (int64_t)a.G * kKvD;         // to the next sequence's heads
                 uint32_t dst = smem_addr(qd + l8 * 16);
 #pragma unroll 1
-                for (int i = 0; i < 8; ++i, dst += 512u) {
+                for (int i = 0; i < steps; ++i, dst += 512u) {
                     const bool in = row0 + 4 * i < a.rows;
                     const float *p = in ? src : a.q;
 #pragma unroll
@@ -867,7 +868,7 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 cp_async_wait<0>();
                 __syncwarp();
 #pragma unroll 2
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < steps; ++i) {
                     float4 v[4];
                     float mx = 0.f;
 #pragma unroll
@@ -880,6 +881,7 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                     const float p2 = pow2_of(mx), inv = inv_pow2(p2) * a.qsign;
                     const float mine = __shfl_sync(0xffffffffu, p2, (lane & 3) * 8);    // also: the rows have been read
                     if (lane >> 2 == i) c2 = fmaxf(a.cscale * mine, 1.17549435e-38f);   // not 0: a masked score is -inf c2
+                    if (g.nt == 1 && l8 == 0) c_of[first_row + 4 * i + sub] = fmaxf(a.cscale * p2, 1.17549435e-38f);
                     const uint32_t row7 = (uint32_t)(sub + 4 * i) & 7u;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -893,13 +895,12 @@ kv_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                             make_uint2(pack_h2(y[0] - h4[0], y[1] - h4[1]), pack_h2(y[2] - h4[2], y[3] - h4[3]));
                     }
                 }
-                if (g.nt == 1) c_of[r] = c2;                       // for buffer 1, which has the same rows
             }
             fence_proxy_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
             bool ok = true;
-            if (g.nt == 1 && b == 1) {
+            if (g.nt == 1) {                                       // both buffers have all the rows
                 ok = __all_sync(0xffffffffu, wait_or_abort(q_full, pq, abort_flag));
                 c2 = c_of[r];
             }
@@ -1288,17 +1289,7 @@ size_t plan(const li_kv_cache *C, int n_q_heads, KvAttnArgs *a, size_t *off /* [
     }
     const int64_t most = pairs * ((a->max_ctx + (int64_t)a->lead + kOwnTok - 1) / kOwnTok);
     if (most >= (1ll << 30) || pairs * a->G >= (1ll << 30) || a->max_ctx + (int64_t)a->lead >= (1ll << 30)) return 0;
-    int64_t grid = most / kOwnMinSteps;
-    grid = grid < 1 ? 1 : grid < sms ? grid : sms;
-    a->own_warps = (int)grid * kOwnWarps;
-    size_t at = 0;
-    off[0] = at; at += al256(((size_t)a->B + 1) * 4);
-    const size_t own_recs = (size_t)pairs + a->own_warps;
-    off[1] = at; at += al256(own_recs * a->G * sizeof(float2));
-    off[2] = at; at += al256(own_recs * a->G * kKvD * 4);
-    a->score_stride = (a->max_ctx + 3) / 4 * 4;
-    off[3] = at; at += C->weight ? al256((size_t)a->B * a->Hq * a->score_stride * 4) : 0;
-    off[4] = off[5] = at;
+    int free_sms = sms;
     if (a->n_prefix > 0) {
         a->rows = a->B * a->G;
         a->n_rt = (a->rows + kPreRows - 1) / kPreRows;
@@ -1309,7 +1300,24 @@ size_t plan(const li_kv_cache *C, int n_q_heads, KvAttnArgs *a, size_t *off /* [
         a->per_group = a->n_rt > 1 && cost >= 2ll * sms ? 2 : 1;
         a->n_grp = (a->n_rt + a->per_group - 1) / a->per_group;
         a->slots = a->per_group == 2 ? kPreSlots2 : kPreSlots1;
-        a->pre_ctas = (int)(cost < sms ? cost : sms);
+        // With little to do, two token tiles a block: a tile for each score buffer, and SMs left for kv_own meanwhile
+        // (16 x 2085 and weights: 29 us with a tile a block on 136 SMs, 24 with two on 68)
+        const int64_t blocks = a->per_group == 1 ? (cost + 1) / 2 : cost;
+        a->pre_ctas = (int)(blocks < sms ? blocks : sms);
+        if (2 * a->pre_ctas <= sms) free_sms = sms - a->pre_ctas;
+    }
+    int64_t grid = most / kOwnMinSteps;
+    grid = grid < 1 ? 1 : grid < free_sms ? grid : free_sms;
+    a->own_warps = (int)grid * kOwnWarps;
+    size_t at = 0;
+    off[0] = at; at += al256(((size_t)a->B + 1) * 4);
+    const size_t own_recs = (size_t)pairs + a->own_warps;
+    off[1] = at; at += al256(own_recs * a->G * sizeof(float2));
+    off[2] = at; at += al256(own_recs * a->G * kKvD * 4);
+    a->score_stride = (a->max_ctx + 3) / 4 * 4;
+    off[3] = at; at += C->weight ? al256((size_t)a->B * a->Hq * a->score_stride * 4) : 0;
+    off[4] = off[5] = at;
+    if (a->n_prefix > 0) {
         const size_t recs = ((size_t)a->Hkv * a->n_grp + a->pre_ctas) * 2 * kPreRows;
         off[4] = at; at += al256(recs * sizeof(float2));
         off[5] = at; at += al256(recs * kKvD * 4);
