@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv_select_kernel(Evic
         }
         return;
     }
-    if (n <= a.budget) {
+    if (n <= a.budget || a.budget == 0) {          // nothing to free, or nothing to keep: no rows move
         if (tid == 0) a.count[pair] = 0;
         return;
     }
@@ -154,7 +154,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv_select_kernel(Evic
             const int x = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += x;
         }
-        if (tid == 0) { s_digit = kBins - 1; s_want = s_all = want; }      // want 0: nothing is kept
         int total, before = warp_offsets<W>(__shfl_sync(0xffffffffu, incl, 31), buf, total) + incl - sum;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
@@ -169,7 +168,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv_select_kernel(Evic
         prefix |= ((uint32_t)s_digit & digits) << shift;
         mask |= digits << shift;
         want = s_want;
+        const bool whole = s_all == want;          // all keys with these digits are kept: the others do not matter
         __syncthreads();
+        if (whole) break;
     }
     // keys above `prefix` are kept, of those equal to it the first `want` (all
     // of them, unless weights are tied at the border): a bit per slot. A warp
@@ -235,12 +236,19 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv_select_kernel(Evic
     if (tid == 0) a.count[pair] = moves;
     __syncthreads();
     const int here = min(moves, kSelMoves);
-    for (int m = tid; m < here; m += THREADS) {
-        const size_t at = (size_t)pair * a.max_ctx;
-        a.weight_rw[at + mine[m].y] = w[mine[m].x];
-        a.slot_pos_rw[at + mine[m].y] = sp[mine[m].x];
+    static_assert(kSelMoves <= THREADS, "a move's weight and position a thread");
+    float wv = 0.f;
+    int32_t pv = 0;
+    if (tid < here) {                              // on their way while the rows move
+        wv = w[mine[tid].x];
+        pv = sp[mine[tid].x];
     }
     move_rows(a, pair, [&](int m) { return mine[m]; }, warp, here, W, lane);
+    if (tid < here) {
+        const size_t at = (size_t)pair * a.max_ctx + mine[tid].y;
+        a.weight_rw[at] = wv;
+        a.slot_pos_rw[at] = pv;
+    }
 }
 
 constexpr int kMoveWarps = 8;

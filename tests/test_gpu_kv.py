@@ -552,6 +552,27 @@ def test_evict_weights(cuda, kind):
     _evict_check(cuda, r, 3, 777, 2, [777, 700, 400], 399, 3, 50, weights, shuffle=kind != "descending")
 
 
+@pytest.mark.parametrize("budget,pos_of", [(0, -1), (0, 10**9), (16, -1), (16, 2**31 - 1), (16, -2**31), (40, 10**9)])
+def test_evict_positions_that_protect_everything(cuda, budget, pos_of):
+    """Positions that no token has (a table that was never filled): all slots
+    protected, so ties go to the lowest; a budget of 0 keeps none even so."""
+    import torch
+    from leaninfer_b200 import ops
+    from oracle import kv
+    r = rng(760)
+    c, t, cache = _cache(r, cuda, 2, 50, 2, [50, 30], stale=7.0)
+    c["slot_pos"][:] = pos_of
+    t["slot_pos"].fill_(pos_of)
+    pos = np.array([49, 29], np.int32)
+    cache.evict(T(pos, cuda), budget, n_sink=0, n_recent=0)
+    lens = c["lens"].copy()
+    kv.evict(c["k"], c["v"], c["weight"], c["slot_pos"], lens, pos, budget, 0, 0)
+    assert np.array_equal(t["lens"].cpu().numpy(), lens)
+    for a, b in ((t["k"], c["k"]), (t["v"], c["v"])):
+        assert np.array_equal(a.cpu().numpy().view(np.uint16), b.view(np.uint16))
+    assert np.array_equal(t["weight"].cpu().numpy(), c["weight"]) and ops.device_status() == 0
+
+
 def test_decode_evict_append_run(cuda):
     """A bounded cache in use: steps of append, decode (weights accumulate)
     and, whenever the cache is full, eviction back to the budget, over a shared
