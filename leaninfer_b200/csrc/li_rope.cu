@@ -9,8 +9,11 @@
 // its tokens' pairs once into shared memory and uses them for every head.
 // A thread's unit of work is two vectors of E values (16 bytes each where
 // alignment and sizes allow): the two halves of E pairs in the half layout,
-// 2E neighbouring values in the interleaved one, so that the layouts differ
-// only in which values of the unit form a pair. A thread keeps its place in
+// two vectors of E / 2 pairs half the rotated part apart in the interleaved
+// one, and two as far apart in the part that passes through, so that the
+// threads of a load or store have neighbouring vectors (neighbours in one
+// thread put the halves of a 32-byte sector into two instructions, 1.8 times the
+// L2 traffic: 47 us for the f16 prompts that take 39). A thread keeps its place in
 // the head and walks over heads and tokens (no division per unit); the first
 // units' loads are issued before the
 // angles are computed, which hides the one behind the other.
@@ -124,6 +127,33 @@ __device__ __forceinline__ void store_pack(O *p, const float (&f)[E]) {
     *reinterpret_cast<V *>(p) = *reinterpret_cast<V *>(&r);
 }
 
+// A block's table of (cos, sin): two pairs are 16 bytes, and the 16-byte groups
+// that a vector takes (kGroups of them) lie a stride apart, so that the threads
+// of a read have neighbouring ones (in pair order they fell on a quarter of the
+// banks). Place of pair i of `half`:
+template <int E, bool HALF> struct Table {
+    static constexpr int kPairs = HALF ? E : E / 2;                    // of a vector
+    static constexpr int kGroups = kPairs >= 2 ? kPairs / 2 : 0;       // 0: pair order
+    static __device__ __forceinline__ int place(int i, int half) {
+        if (kGroups <= 1) return i;
+        const int g = i >> 1;
+        return 2 * ((g % (kGroups ? kGroups : 1)) * (half / kPairs) + g / (kGroups ? kGroups : 1)) + (i & 1);
+    }
+    // pairs of vector v
+    static __device__ __forceinline__ void read(const float2 *t, int v, int half, float2 (&c)[kPairs ? kPairs : 1]) {
+        if (kGroups == 0) {
+            c[0] = t[v];
+        } else {
+#pragma unroll
+            for (int k = 0; k < kGroups; ++k) {
+                const float4 x = reinterpret_cast<const float4 *>(t)[k * (half / kPairs) + v];
+                c[2 * k] = make_float2(x.x, x.y);
+                c[2 * k + 1] = make_float2(x.z, x.w);
+            }
+        }
+    }
+};
+
 template <typename T, int E, bool HALF, bool APPEND>
 __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_kernel(const __grid_constant__ RopeJob j) {
     extern __shared__ __align__(16) uint8_t rope_smem[];
@@ -138,8 +168,8 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_kernel(const _
     // this thread's place: unit u of head hd (of hp heads), the same in every round
     const int hd = threadIdx.x / j.units, u = threadIdx.x - hd * j.units;
     const bool rot = u < j.n_rot, worker = hd < j.hp;
-    const int oa = rot ? (HALF ? u * E : u * 2 * E) : j.r.rope_dim + (u - j.n_rot) * 2 * E;
-    const int ob = rot && HALF ? half + u * E : oa + E;
+    const int oa = !rot ? j.r.rope_dim + (u - j.n_rot) * E : !HALF && E == 1 ? 2 * u : u * E;
+    const int ob = !rot ? oa + (j.units - j.n_rot) * E : !HALF && E == 1 ? oa + 1 : half + oa;
     const bool two = ob < j.D;
     // a walk over (token, round): the unit at (t, p) is head h0 + hd + p hp of token t0 + t
     struct Walk { int t, p; };
@@ -168,7 +198,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_kernel(const _
                 const int tok = i / half;
                 float2 x = rope_cos_sin(j.r, j.pos[t0 + tok], i - tok * half);
                 x.y *= j.sin_sign;
-                cs[i] = x;
+                cs[tok * half + Table<E, HALF>::place(i - tok * half, half)] = x;
             }
             if (APPEND && (int)threadIdx.x < nt) {
                 const int t = t0 + threadIdx.x, s = j.seq ? j.seq[t] : t;
@@ -194,16 +224,30 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_kernel(const _
                 x[1][e] = two ? to_f(b[i].v[e]) : 0.f;
             }
             if (rot && (!APPEND || h < j.Hq + j.Hkv)) {
-                const float2 *cp = cs + wk.t * half + u * E;
+                const float2 *cp = cs + wk.t * half;
+                constexpr int P = Table<E, HALF>::kPairs;
+                if (HALF || E == 1) {              // pair e: (a_e, b_e)
+                    float2 c[HALF ? E : 1];
+                    if constexpr (HALF) Table<E, HALF>::read(cp, u, half, c);
+                    else c[0] = cp[u];
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    // pair e of the unit: (a_e, b_e), or values 2e and 2e + 1 of the 2E neighbours
-                    float &lo = HALF ? x[0][e] : x[(2 * e) / E][(2 * e) % E];
-                    float &hi = HALF ? x[1][e] : x[(2 * e + 1) / E][(2 * e + 1) % E];
-                    const float p = lo, q = hi;
-                    const float2 c = cp[e];
-                    lo = p * c.x - q * c.y;
-                    hi = q * c.x + p * c.y;
+                    for (int e = 0; e < E; ++e) {
+                        const float p = x[0][e], q = x[1][e];
+                        x[0][e] = p * c[e].x - q * c[e].y;
+                        x[1][e] = q * c[e].x + p * c[e].y;
+                    }
+                } else if constexpr (P > 0) {      // pairs of neighbours in a (vector u) and in b (vector u + n_rot)
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        float2 c[P];
+                        Table<E, HALF>::read(cp, u + v * j.n_rot, half, c);
+#pragma unroll
+                        for (int e = 0; e < P; ++e) {
+                            const float p = x[v][2 * e], q = x[v][2 * e + 1];
+                            x[v][2 * e] = p * c[e].x - q * c[e].y;
+                            x[v][2 * e + 1] = q * c[e].x + p * c[e].y;
+                        }
+                    }
                 }
             }
             if (!APPEND || h < j.Hq) {
