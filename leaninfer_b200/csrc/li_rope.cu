@@ -132,15 +132,16 @@ __device__ __forceinline__ void store_pack(O *p, const float (&f)[E]) {
 // of a read have neighbouring ones (in pair order they fell on a quarter of the
 // banks). Place of pair i of `half`:
 template <int E, bool HALF> struct Table {
-    static constexpr int kPairs = HALF ? E : E / 2;                    // of a vector
-    static constexpr int kGroups = kPairs >= 2 ? kPairs / 2 : 0;       // 0: pair order
+    static constexpr int kPairs = HALF ? E : E > 1 ? E / 2 : 1;        // of a vector (E 1, interleaved: of two)
+    static constexpr int kGroups = kPairs / 2;                         // 0: pair order
     static __device__ __forceinline__ int place(int i, int half) {
-        if (kGroups <= 1) return i;
+        constexpr int K = kGroups > 1 ? kGroups : 1;
+        if (K == 1) return i;
         const int g = i >> 1;
-        return 2 * ((g % (kGroups ? kGroups : 1)) * (half / kPairs) + g / (kGroups ? kGroups : 1)) + (i & 1);
+        return 2 * ((g % K) * (half / kPairs) + g / K) + (i & 1);
     }
     // pairs of vector v
-    static __device__ __forceinline__ void read(const float2 *t, int v, int half, float2 (&c)[kPairs ? kPairs : 1]) {
+    static __device__ __forceinline__ void read(const float2 *t, int v, int half, float2 (&c)[kPairs]) {
         if (kGroups == 0) {
             c[0] = t[v];
         } else {
@@ -226,17 +227,16 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_kernel(const _
             if (rot && (!APPEND || h < j.Hq + j.Hkv)) {
                 const float2 *cp = cs + wk.t * half;
                 constexpr int P = Table<E, HALF>::kPairs;
-                if (HALF || E == 1) {              // pair e: (a_e, b_e)
-                    float2 c[HALF ? E : 1];
-                    if constexpr (HALF) Table<E, HALF>::read(cp, u, half, c);
-                    else c[0] = cp[u];
+                if constexpr (HALF || E == 1) {    // pair e: (a_e, b_e)
+                    float2 c[P];
+                    Table<E, HALF>::read(cp, u, half, c);
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
                         const float p = x[0][e], q = x[1][e];
                         x[0][e] = p * c[e].x - q * c[e].y;
                         x[1][e] = q * c[e].x + p * c[e].y;
                     }
-                } else if constexpr (P > 0) {      // pairs of neighbours in a (vector u) and in b (vector u + n_rot)
+                } else {                           // pairs of neighbours in a (vector u) and in b (vector u + n_rot)
 #pragma unroll
                     for (int v = 0; v < 2; ++v) {
                         float2 c[P];
