@@ -99,7 +99,7 @@ struct KvAttnArgs {
     float2 *pre_ml;                    // [Hkv n_grp + pre_ctas][2][128 rows]
     float *pre_o;                      // [Hkv n_grp + pre_ctas][2][32 groups of 4 dims][128 rows][4]
     // join
-    int row_ctas, wpr, w_chunks;       // blocks that join rows, warps per 4 rows, blocks per pair that write weights
+    int row_ctas, wpr, w_chunks;       // blocks that join rows, warps per row block, blocks per pair that write weights
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -1027,12 +1027,12 @@ struct RowPieces {
     int rec0, gq;                          // own
 };
 
-__device__ __forceinline__ RowPieces pieces_of(const KvAttnArgs &a, int j, int row) {
+// The prefix's share follows from the sizes alone; the sequences' own shares
+// wait for kv_own's table.
+__device__ __forceinline__ RowPieces prefix_pieces(const KvAttnArgs &a, int j, int row) {
     RowPieces x;
-    const int s = row / a.G;
-    x.gq = row - s * a.G;
+    x.gq = row % a.G;
     x.n_pre = x.n_own = 0;
-    const int n = own_tokens(a, s), T = __ldcg(a.base + a.B), b0 = __ldcg(a.base + s);
     if (a.n_prefix > 0) {
         const int rt = row / kPreRows;
         x.prow = row - rt * kPreRows;
@@ -1047,6 +1047,11 @@ __device__ __forceinline__ RowPieces pieces_of(const KvAttnArgs &a, int j, int r
         x.stream0 = g.nt == 2 ? rt - g.rt : 0;
         x.n_pre = (c1 - x.c0 + 1) * x.streams;
     }
+    return x;
+}
+
+__device__ __forceinline__ void own_pieces(const KvAttnArgs &a, RowPieces &x, int j, int s) {
+    const int n = own_tokens(a, s), T = __ldcg(a.base + a.B), b0 = __ldcg(a.base + s);
     if (n > 0) {
         const Runs runs(T, own_active(T, a.own_warps));
         const int st = own_steps(n), at = b0 + j * st;
@@ -1054,7 +1059,6 @@ __device__ __forceinline__ RowPieces pieces_of(const KvAttnArgs &a, int j, int r
         x.rec0 = s * a.Hkv + j + w0;
         x.n_own = w1 - w0 + 1;
     }
-    return x;
 }
 
 // Record of prefix piece i, or -1 where that piece holds no token.
@@ -1075,38 +1079,44 @@ __device__ __forceinline__ float2 piece_ml(const KvAttnArgs &a, const RowPieces 
     return __ldcg(a.own_ml + (size_t)(x.rec0 + i - x.n_pre) * a.G + x.gq);
 }
 
-constexpr int kJoinWarps = 8, kJoinRows = 4;
+constexpr int kJoinWarps = 8;
 constexpr int kJoinRun = kJoinWarps * kWarp * 4;     // slots of a weight block's step
 
-// Rows: wpr neighbouring warps take 4 rows of a kv head, each its share of the
-// pieces; lane l holds row l % 4 and dims 32 i + 4 (l / 4) .. +3, i < 4 (the
-// prefix's records lie dims first, so a load reads whole sectors either way).
+// Rows: wpr neighbouring warps take ROWS rows of a kv head, each its share of
+// the pieces; lane l holds row l % ROWS and the 4-dim groups l / ROWS,
+// + 32 / ROWS, ... (the prefix's records lie dims first, so that with four rows
+// a load reads whole sectors either way). With one row a warp has eight pieces
+// in flight instead of two: few rows with many pieces each (one sequence's
+// long cache is cut into hundreds).
+template <int ROWS>
 __global__ void __launch_bounds__(kJoinWarps * kWarp, 3) kv_join_kernel(const __grid_constant__ KvAttnArgs a) {
-    __shared__ float red_m[kJoinWarps][kJoinRows], red_l[kJoinWarps][kJoinRows];
-    __shared__ __align__(16) float4 red_o[kJoinWarps][4][kWarp];
+    constexpr int kPer = 8 / ROWS, kApart = kWarp / ROWS;
+    __shared__ float red_m[kJoinWarps][ROWS], red_l[kJoinWarps][ROWS];
+    __shared__ __align__(16) float4 red_o[kJoinWarps][ROWS][kWarp];
     __shared__ float gm[16], gi[16];
-    grid_dep_wait();
-    grid_dep_launch_dependents();
     const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
     if ((int)blockIdx.x < a.row_ctas) {
         const int per = kJoinWarps / a.wpr, sub = warp % a.wpr;
-        const int rows = a.B * a.G, blocks = (rows + kJoinRows - 1) / kJoinRows;      // row blocks of a kv head
+        const int rows = a.B * a.G, blocks = (rows + ROWS - 1) / ROWS;      // row blocks of a kv head
         const int item = blockIdx.x * per + warp / a.wpr, j = item / blocks;
-        const int rl = lane & 3, xq = lane >> 2, row = (item - j * blocks) * kJoinRows + rl;
+        const int rl = lane % ROWS, xq = lane / ROWS, row = (item - j * blocks) * ROWS + rl;
         const bool on = j < a.Hkv && row < rows;
+        RowPieces x = prefix_pieces(a, on ? j : 0, on ? row : 0);
+        grid_dep_wait();
+        grid_dep_launch_dependents();
         float m = -INFINITY, l = 0.f;
-        float4 o[4];
+        float4 o[ROWS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < ROWS; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (on) {
-            const RowPieces x = pieces_of(a, j, row);
+            own_pieces(a, x, j, row / a.G);
             const int n = x.n_pre + x.n_own;
-            // two pieces at a time, their loads in flight together (predicated, not branched over)
-            for (int i0 = sub; i0 < n; i0 += 2 * a.wpr) {
-                float4 v[2][4];
-                float2 ml[2];
+            // kPer pieces at a time, their loads in flight together (predicated, not branched over)
+            for (int i0 = sub; i0 < n; i0 += kPer * a.wpr) {
+                float4 v[kPer][ROWS];
+                float2 ml[kPer];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
+                for (int e = 0; e < kPer; ++e) {
                     const int i = i0 + e * a.wpr;
                     const bool pre = i < x.n_pre;
                     const int rec = i >= n ? -1 : pre ? pre_record(a, x, i) : (x.rec0 + i - x.n_pre) * a.G + x.gq;
@@ -1114,32 +1124,36 @@ __global__ void __launch_bounds__(kJoinWarps * kWarp, 3) kv_join_kernel(const __
                                                   ((size_t)max(rec, 0) * 32 + xq) * kPreRows + x.prow
                                             : reinterpret_cast<const float4 *>(a.own_o) + (size_t)max(rec, 0) * 32 + xq;
                     const float2 *mp = pre ? a.pre_ml + (size_t)max(rec, 0) * kPreRows + x.prow : a.own_ml + max(rec, 0);
-                    const int step = pre ? 8 * kPreRows : 8;
+                    const int step = pre ? kApart * kPreRows : kApart;
                     ml[e] = rec >= 0 ? __ldcg(mp) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
+                    for (int k = 0; k < ROWS; ++k)
                         v[e][k] = rec >= 0 ? __ldcg(src + k * step) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
-                const float mx = fmaxf(m, fmaxf(ml[0].x, ml[1].x));
+                float mx = m;
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) mx = fmaxf(mx, ml[e].x);
                 const float keep = m == -INFINITY ? 0.f : ex2(m - mx);
-                float f[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) f[e] = ml[e].x == -INFINITY ? 0.f : ex2(ml[e].x - mx);
                 m = mx;
-                l = fmaf(f[0], ml[0].y, fmaf(f[1], ml[1].y, l * keep));
+                l *= keep;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    o[k].x = fmaf(f[0], v[0][k].x, fmaf(f[1], v[1][k].x, o[k].x * keep));
-                    o[k].y = fmaf(f[0], v[0][k].y, fmaf(f[1], v[1][k].y, o[k].y * keep));
-                    o[k].z = fmaf(f[0], v[0][k].z, fmaf(f[1], v[1][k].z, o[k].z * keep));
-                    o[k].w = fmaf(f[0], v[0][k].w, fmaf(f[1], v[1][k].w, o[k].w * keep));
+                for (int k = 0; k < ROWS; ++k) { o[k].x *= keep; o[k].y *= keep; o[k].z *= keep; o[k].w *= keep; }
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    const float f = ml[e].x == -INFINITY ? 0.f : ex2(ml[e].x - mx);
+                    l = fmaf(f, ml[e].y, l);
+#pragma unroll
+                    for (int k = 0; k < ROWS; ++k) {
+                        o[k].x = fmaf(f, v[e][k].x, o[k].x); o[k].y = fmaf(f, v[e][k].y, o[k].y);
+                        o[k].z = fmaf(f, v[e][k].z, o[k].z); o[k].w = fmaf(f, v[e][k].w, o[k].w);
+                    }
                 }
             }
         }
         if (a.wpr > 1) {
             if (xq == 0) { red_m[warp][rl] = m; red_l[warp][rl] = l; }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) red_o[warp][k][lane] = o[k];
+            for (int k = 0; k < ROWS; ++k) red_o[warp][k][lane] = o[k];
             __syncthreads();
             if (sub == 0) {
                 float M = m;
@@ -1148,7 +1162,7 @@ __global__ void __launch_bounds__(kJoinWarps * kWarp, 3) kv_join_kernel(const __
                     const float f = red_m[warp + w][rl] == -INFINITY ? 0.f : ex2(red_m[warp + w][rl] - M);
                     l = w ? fmaf(f, red_l[warp + w][rl], l) : f * l;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
+                    for (int k = 0; k < ROWS; ++k) {
                         const float4 v = red_o[warp + w][k][lane];
                         o[k].x = w ? fmaf(f, v.x, o[k].x) : f * v.x; o[k].y = w ? fmaf(f, v.y, o[k].y) : f * v.y;
                         o[k].z = w ? fmaf(f, v.z, o[k].z) : f * v.z; o[k].w = w ? fmaf(f, v.w, o[k].w) : f * v.w;
@@ -1162,24 +1176,27 @@ __global__ void __launch_bounds__(kJoinWarps * kWarp, 3) kv_join_kernel(const __
             const int s = row / a.G;
             float4 *d = reinterpret_cast<float4 *>(a.out + ((size_t)s * a.Hq + (size_t)j * a.G + row - s * a.G) * kKvD) + xq;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < ROWS; ++k) {
                 float4 v = make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv);
                 if (a.gate) {
                     const float4 gt = reinterpret_cast<const float4 *>(
-                        a.gate + s * a.gate_stride + ((size_t)j * a.G + row - s * a.G) * kKvD)[xq + 8 * k];
+                        a.gate + s * a.gate_stride + ((size_t)j * a.G + row - s * a.G) * kKvD)[xq + kApart * k];
                     v.x *= sigmoid(gt.x); v.y *= sigmoid(gt.y); v.z *= sigmoid(gt.z); v.w *= sigmoid(gt.w);
                 }
-                d[8 * k] = v;
+                d[kApart * k] = v;
             }
         }
         return;
     }
+    grid_dep_wait();
+    grid_dep_launch_dependents();
     // weights of the pair (s, j), every w_chunks-th run of slots, four neighbouring ones a thread
     const int item = blockIdx.x - a.row_ctas, pair = item / a.w_chunks, chunk = item - pair * a.w_chunks;
     const int s = pair / a.Hkv, j = pair - s * a.Hkv, n = own_len(a, s);
     if (chunk * kJoinRun >= n) return;
     for (int gq = warp; gq < a.G; gq += kJoinWarps) {
-        const RowPieces x = pieces_of(a, j, s * a.G + gq);
+        RowPieces x = prefix_pieces(a, j, s * a.G + gq);
+        own_pieces(a, x, j, s);
         const int cnt = x.n_pre + x.n_own;
         float m = -INFINITY, l = 0.f;
         for (int i = lane; i < cnt; i += kWarp) {
@@ -1301,8 +1318,9 @@ size_t plan(const li_kv_cache *C, int n_q_heads, KvAttnArgs *a, size_t *off /* [
         a->n_grp = (a->n_rt + a->per_group - 1) / a->per_group;
         a->slots = a->per_group == 2 ? kPreSlots2 : kPreSlots1;
         // With little to do, two token tiles a block: a tile for each score buffer, and SMs left for kv_own meanwhile
-        // (16 x 2085 and weights: 29 us with a tile a block on 136 SMs, 24 with two on 68)
-        const int64_t blocks = a->per_group == 1 ? (cost + 1) / 2 : cost;
+        // (16 x 2085 and weights: 29 us with a tile a block on 136 SMs, 24 with two on 68). A prefix of one tile has
+        // no second one to add: a block a group (28 us from 34 at 201 x 123 x 16 heads).
+        const int64_t blocks = a->per_group == 1 && a->n_tt > 1 ? (cost + 1) / 2 : cost;
         a->pre_ctas = (int)(blocks < sms ? blocks : sms);
         if (2 * a->pre_ctas <= sms) free_sms = sms - a->pre_ctas;
     }
@@ -1409,12 +1427,16 @@ int li::attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_stride, i
     if (a.G <= 8) rc = a.weight ? launch_own<1, true>(a, st) : launch_own<1, false>(a, st);
     else rc = a.weight ? launch_own<2, true>(a, st) : launch_own<2, false>(a, st);
     if (rc) return rc;
-    // warps per 4 rows: as many as it takes to fill the SMs, up to the pieces that a row can have
+    // A row a warp where eight warps a row do not fill the SMs twice over, four rows where they do (a row a warp: 45 us
+    // from 54 at 27 sequences x 40775 x 6 heads, 31 from 52 at 5 x 9910 x 16; 1 us behind at 180 rows with few
+    // pieces, and 25 against 23 at 512 rows); and as many warps on them as it takes to fill the SMs, up to the pieces
+    // that a row can have.
     const int pairs = a.B * a.Hkv;
     const int64_t pre = a.n_prefix ? 2ll * a.pre_ctas / (a.Hkv * a.n_grp) + 2 : 0;
     int64_t own = (a.max_ctx + (int64_t)a.lead + kOwnTok - 1) / kOwnTok / kOwnMinSteps + 1;
     if (own > a.own_warps / pairs + 2) own = a.own_warps / pairs + 2;
-    const int64_t row_blocks = (int64_t)a.Hkv * ((a.B * a.G + kJoinRows - 1) / kJoinRows);
+    const int rows_each = (int64_t)pairs * a.G <= 2ll * num_sms() ? 1 : 4;
+    const int64_t row_blocks = (int64_t)a.Hkv * ((a.B * a.G + rows_each - 1) / rows_each);
     a.wpr = 1;
     while (a.wpr < kJoinWarps && a.wpr < pre + own && row_blocks * a.wpr < 16ll * num_sms()) a.wpr *= 2;
     const int per = kJoinWarps / a.wpr;
@@ -1427,5 +1449,7 @@ int li::attn_kv_decode(const li_kv_cache *C, const float *q, int64_t q_stride, i
         blocks += (int64_t)pairs * a.w_chunks;
     }
     if (blocks > 0x7fffffff) return LI_ERR_BAD_SHAPE;
-    return (int)launch_pdl(kv_join_kernel, dim3((unsigned)blocks), dim3(kJoinWarps * kWarp), 0, st, true, a);
+    return rows_each == 1
+               ? (int)launch_pdl(kv_join_kernel<1>, dim3((unsigned)blocks), dim3(kJoinWarps * kWarp), 0, st, true, a)
+               : (int)launch_pdl(kv_join_kernel<4>, dim3((unsigned)blocks), dim3(kJoinWarps * kWarp), 0, st, true, a);
 }
