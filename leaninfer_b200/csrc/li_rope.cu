@@ -64,9 +64,9 @@ namespace {
 
 constexpr int kRopeThreads = 256;      // at most
 // Units of a thread in flight, and blocks per SM that the registers are held
-// down to: more of the one costs the other. Two and four took 24.9 us for 4096
-// tokens x 48 heads x 128 bf16 (of 15.6 at the copy rate), four units without
-// a bound 36 us, three 33 us, two at five blocks 30 us.
+// down to: more of the one costs the other. Two and four take 22.8 us for 4096
+// tokens x 48 heads x 128 bf16 (of 15.6 at the copy rate), three units at four
+// blocks 31 us, four at three 33 us, two at five blocks 29 us.
 constexpr int kRopeBatch = 2, kRopeBlocks = 4;
 
 // One launch over n_tokens tokens and `heads` head slots. Plain rotation: one
