@@ -388,6 +388,34 @@ def test_large_prefix_variants(cuda, kw):
     _attn_check(cuda, rng(600), 20, 1700, 70, [(i * 13) % 71 for i in range(20)], 2, 5, **kw)
 
 
+# On both sides of 296 rows the join takes its rows differently: one a warp, four a warp.
+ROWS = [
+    # B, P, ctx, lens, Hkv, G
+    (5, 9910, 3, [0, 1, 2, 2, 0], 1, 16),                     # few rows, hundreds of pieces each
+    (1, 20011, 9, [4], 1, 1),
+    (27, 6001, 300, [i * 11 for i in range(27)], 2, 3),
+    (37, 1700, 64, [i + 7 for i in range(37)], 1, 8),         # 296 rows
+    (99, 1000, 20, [i % 21 for i in range(99)], 1, 3),        # 297
+    (201, 123, 1, [i % 2 for i in range(201)], 4, 2),         # a prefix of one token tile, four row tiles
+    (60, 0, 1500, [1500 - 25 * i for i in range(60)], 1, 8),  # four rows a warp, many pieces each
+]
+
+
+@pytest.mark.parametrize("case", range(len(ROWS)))
+def test_attention_joins_few_and_many_rows(cuda, case):
+    B, P, ctx, lens, Hkv, G = ROWS[case]
+    _attn_check(cuda, rng(620 + case), B, P, ctx, lens, Hkv, G, decay=[1.0, 0.0, 0.75][case % 3])
+
+
+@pytest.mark.parametrize("kw", [
+    dict(weight=False), dict(gap=20), dict(q_scale=0.0), dict(scale=0.0), dict(scale=-0.3), dict(graph=True),
+    dict(graph=True, weight=False)])
+@pytest.mark.parametrize("P", [0, 900])
+def test_many_rows_variants(cuda, P, kw):
+    """The variants above with 440 rows."""
+    _attn_check(cuda, rng(640), 88, P, 70, [(i * 13) % 71 for i in range(88)], 1, 5, **kw)
+
+
 def test_large_prefix_growing_scores(cuda):
     """Scores that rise along the prefix by far more than the lag of the
     running maximum, and fall, and jump: every rescaling path."""
