@@ -304,6 +304,7 @@ int rope_launch(RopeJob &j, int e_max, cudaStream_t s) {
         j.tb = (int)(share / per_tok);
         const int tb_max = 16384 / (8 + 4 * j.r.rope_dim);              // 16 KB of angles
         if (j.tb > tb_max) j.tb = tb_max;
+        if (j.tb > kRopeThreads) j.tb = kRopeThreads;                   // small heads: a thread holds one token's row
         if (j.tb > j.n_tokens) j.tb = j.n_tokens;
     }
     j.n_hblk = (j.heads + j.hb - 1) / j.hb;

@@ -642,3 +642,25 @@ def test_decode_evict_append_run(cuda):
             kept = host["slot_pos"][:, :, :n]
             assert (kept < P + 2).sum() == B * Hkv * 2 and (kept > pos[0] - 5).sum() == B * Hkv * 5
     assert ops.device_status() == 0
+
+
+# --------------------------------------------------------------------------
+@pytest.mark.parametrize("dt,head_dim,rope_dim,heads,layout", [
+    ("f32", 8, 8, 1, "half"), ("f32", 16, 8, 1, "interleaved"), ("bf16", 16, 8, 1, "half"), ("bf16", 2, 2, 2, "half"),
+    ("f16", 2, 2, 1, "interleaved"), ("bf16", 32, 0, 1, "half"), ("f16", 8, 4, 3, "interleaved"),
+    ("f32", 48, 12, 1, "half")])
+def test_rope_of_small_heads_over_many_tokens(cuda, dt, head_dim, rope_dim, heads, layout):
+    """One to three small heads a token: blocks take hundreds of tokens, which
+    is more tokens than a block has threads."""
+    from leaninfer_b200 import ops
+    from oracle import kv
+    r = rng(900 + head_dim + heads)
+    tokens = 260011
+    kw = dict(head_dim=head_dim, rope_dim=rope_dim, layout=layout, theta=1e4)
+    x = T(r.standard_normal((tokens, heads, head_dim)).astype(np.float32), cuda).to(_torch_dt(dt))
+    pos = r.integers(0, 1 << 20, tokens).astype(np.int32)
+    x64 = x.double().cpu().numpy()
+    R = ops.Rope(**kw)
+    _check_rope(ops.rope(R, x, T(pos, cuda)), kv.rope(x64, pos, **kw), x64, 1.0, dt)
+    _check_rope(ops.rope(R, x, T(pos, cuda), out=x), kv.rope(x64, pos, **kw), x64, 1.0, dt, "in place")
+    assert ops.device_status() == 0
