@@ -118,10 +118,12 @@ __device__ __forceinline__ int own_tokens(const KvAttnArgs &a, int s) { return o
 
 __device__ __forceinline__ int own_steps(int n) { return (n + kOwnTok - 1) / kOwnTok; }
 
-// Power of two 2^e with |x| / 2^e in [1, 2) (1 for 0, infinities and NaN).
+// Power of two 2^e with |x| / 2^e in [1, 2) (1 for infinities and NaN). The
+// exponent stays within -126 .. 126, where 2^-e is a normal float too: below
+// it |x| / 2^e is less than 1, above it in [2, 4), which fits f16 as well.
 __device__ __forceinline__ float pow2_of(float x) {
     const uint32_t e = (__float_as_uint(x) >> 23) & 255u;
-    return e == 0u || e == 255u ? 1.f : __uint_as_float(e << 23);
+    return e == 255u ? 1.f : __uint_as_float(min(max(e, 1u), 253u) << 23);
 }
 
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
@@ -132,11 +134,8 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
 // hi keeps the top 11 bits of x (exact in f16), lo the rest.
 __device__ __forceinline__ float hi_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
-// A row's scale as 1 / 2^e: exact, and finite for every normal 2^e but 2^127.
-__device__ __forceinline__ float inv_pow2(float p) {
-    const uint32_t e = __float_as_uint(p) >> 23;
-    return __uint_as_float((e >= 254u ? 1u : 254u - e) << 23);
-}
+// 1 / 2^e of a power that pow2_of gave: exact.
+__device__ __forceinline__ float inv_pow2(float p) { return __uint_as_float((254u << 23) - __float_as_uint(p)); }
 
 // ---------------------------------------------------------------------------
 // A line of T units dealt to W takers in runs whose lengths differ by at most

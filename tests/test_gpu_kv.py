@@ -664,3 +664,24 @@ def test_rope_of_small_heads_over_many_tokens(cuda, dt, head_dim, rope_dim, head
     _check_rope(ops.rope(R, x, T(pos, cuda)), kv.rope(x64, pos, **kw), x64, 1.0, dt)
     _check_rope(ops.rope(R, x, T(pos, cuda), out=x), kv.rope(x64, pos, **kw), x64, 1.0, dt, "in place")
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("kw", [dict(q_scale=1e38, scale=1.2e-38, k_scale=0.05),
+                                dict(q_scale=1e38, scale=-1.2e-38, k_scale=0.05),
+                                dict(q_scale=1e-40, scale=1e37, k_scale=500.0)])
+@pytest.mark.parametrize("B,P", [(3, 50), (20, 1700)])
+def test_queries_at_the_ends_of_fp32(cuda, B, P, kw):
+    """Rows of q whose largest value is beyond 2^127, or below the normal
+    floats, with scales that leave ordinary scores (30 at most): the row's
+    power of two and its inverse stay exact."""
+    class Clipped:                         # fp32's largest is 3.4e38
+        def __init__(self):
+            self.r = rng(910)
+
+        def __getattr__(self, name):
+            return getattr(self.r, name)
+
+        def standard_normal(self, shape):
+            return np.clip(self.r.standard_normal(shape), -3.3, 3.3)
+
+    _attn_check(cuda, Clipped(), B, P, 70, [(i * 13) % 71 for i in range(B)], 2, 5, **kw)
