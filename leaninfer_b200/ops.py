@@ -325,7 +325,7 @@ class AttnLayerDecode:
         """One decode step on a managed cache: the new token of sequence s, at
         position pos[s] (int32), goes to slot cache.len[s] - 1; rope defaults
         to the layer's own parameters."""
-        _on(cache.index, x, y, pos, workspace)
+        _on(cache.index, x, y, pos, workspace, rope.keep if rope is not None else None, *self.keep)
         if x.shape != (cache.n_seqs, self.L.hidden) or y.shape != x.shape or x.dtype != y.dtype or \
                 x.dtype != torch.float32:
             raise ValueError(f"x, y: expected fp32 [{cache.n_seqs}, {self.L.hidden}]")

@@ -258,3 +258,38 @@ def test_rope_node_checks(lib):
     gone = t(ggml.I32, [5], 4)
     gone.data = None
     assert run(pos=gone) == BAD_ARG
+
+
+class _On:
+    """Stands for a CUDA tensor of a device; nothing reads it."""
+
+    def __init__(self, index, shape=(), dtype=None):
+        self.index, self.shape, self.dtype = index, shape, dtype
+
+    def get_device(self):
+        return self.index
+
+
+def test_layer_step_refuses_tensors_of_another_device(monkeypatch):
+    """Every tensor that a layer step on a managed cache reads: the step's own,
+    the frequency divisors and the layer's weights."""
+    import types
+
+    import torch
+    from leaninfer_b200 import ops
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(ops._lib, "load", lambda: pytest.fail("the call went past the device check"))
+    cache = types.SimpleNamespace(index=0, n_seqs=2)
+
+    def step(where):
+        at = lambda name: 1 if name == where else 0
+        layer = object.__new__(ops.AttnLayerDecode)
+        layer.L = types.SimpleNamespace(hidden=64)
+        layer.keep = [_On(at(n)) if n else None for n in ("w_in", "w_out", "", "q_norm_w", "")]
+        rope = types.SimpleNamespace(keep=_On(at("freq_factors")))
+        x, y = (_On(at(n), (2, 64), torch.float32) for n in ("x", "y"))
+        layer.step_kv(x, y, cache, _On(at("pos")), rope=rope, workspace=_On(at("workspace")))
+
+    for where in ("x", "y", "pos", "workspace", "freq_factors", "w_in", "w_out", "q_norm_w"):
+        with pytest.raises(ValueError, match="one device"):
+            step(where)
