@@ -526,7 +526,8 @@ class KVCache:
         if self.n_seqs == 0:
             return
         lib = _lib.load()
+        # kept at the largest size that any budget needs (half of the slots): one for all of them
         ws = workspace if workspace is not None else self._workspace(
-            ("evict", budget), lambda: int(lib.li_kv_evict_workspace_size(self.ref, budget)))
+            "evict", lambda: int(lib.li_kv_evict_workspace_size(self.ref, self.max_ctx // 2)))
         check(lib.li_launch_kv_evict(self.ref, _index(pos, self.n_seqs, "pos"), budget, n_sink, n_recent,
                                      ws.data_ptr(), ws.numel(), _stream()), "li_launch_kv_evict")

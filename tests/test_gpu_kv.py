@@ -685,3 +685,18 @@ def test_queries_at_the_ends_of_fp32(cuda, B, P, kw):
             return np.clip(self.r.standard_normal(shape), -3.3, 3.3)
 
     _attn_check(cuda, Clipped(), B, P, 70, [(i * 13) % 71 for i in range(B)], 2, 5, **kw)
+
+
+def test_evict_workspace_does_not_grow_with_budgets(cuda):
+    """One workspace serves every budget: a host that varies it allocates no
+    more, and the address that a captured eviction holds stays in use."""
+    import torch
+    r = rng(920)
+    c, t, cache = _cache(r, cuda, 2, 600, 2, [600, 600], stale=None)
+    pos = T(np.full(2, 599, np.int32), cuda)
+    cache.evict(pos, 599)
+    before = torch.cuda.memory_allocated()
+    for budget in (590, 580, 400, 301, 300, 299, 200, 100, 7, 0):
+        cache.evict(pos, budget)
+        assert t["lens"].tolist() == [budget] * 2
+        assert torch.cuda.memory_allocated() == before
