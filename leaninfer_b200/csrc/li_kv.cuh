@@ -22,8 +22,10 @@ inline int check_kv_cache(const li_kv_cache *C) {
     if (C->n_prefix > 0 && (!aligned16(C->k_prefix) || !aligned16(C->v_prefix))) return LI_ERR_MISALIGNED;
     if (((uintptr_t)C->len & 3u) || ((uintptr_t)C->weight & 3u) || ((uintptr_t)C->slot_pos & 3u))
         return LI_ERR_MISALIGNED;
-    // (sequence, kv head, slot) counts stay below 2^40, (sequence, kv head) pairs below 2^31
-    if ((int64_t)C->n_seqs * C->n_kv_heads >= (1ll << 31)) return LI_ERR_BAD_SHAPE;
+    // (sequence, kv head) pairs stay below 2^31, (sequence, kv head, slot) counts below 2^40: more than any device
+    // holds, and no size made of them overflows
+    const int64_t pairs = (int64_t)C->n_seqs * C->n_kv_heads;
+    if (pairs >= (1ll << 31) || pairs * C->max_ctx >= (1ll << 40)) return LI_ERR_BAD_SHAPE;
     return 0;
 }
 

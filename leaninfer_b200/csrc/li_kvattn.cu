@@ -1299,7 +1299,7 @@ size_t plan(const li_kv_cache *C, int n_q_heads, KvAttnArgs *a, size_t *off /* [
     const int64_t pairs = (int64_t)a->B * a->Hkv;
     // A prefix that is little to read even once per sequence (30 MB: about 5 us), or that has one reader, goes with
     // the own tokens: one kernel less, and no tile of 128 rows for a few.
-    if (a->n_prefix > 0 && (a->B == 1 || pairs * a->n_prefix * (4ll * kKvD) <= (30ll << 20))) {
+    if (a->n_prefix > 0 && (a->B == 1 || pairs * a->n_prefix <= (30ll << 20) / (4 * kKvD))) {
         a->lead = a->n_prefix;
         a->n_prefix = 0;
     }

@@ -293,3 +293,15 @@ def test_layer_step_refuses_tensors_of_another_device(monkeypatch):
     for where in ("x", "y", "pos", "workspace", "freq_factors", "w_in", "w_out", "q_norm_w"):
         with pytest.raises(ValueError, match="one device"):
             step(where)
+
+
+@pytest.mark.parametrize("n_seqs,heads,ctx", [(1 << 15, 1 << 10, 1 << 15), (1 << 20, 1, 1 << 20),
+                                              ((1 << 31) - 1, 1, (1 << 31) - 1), (1, (1 << 31) - 1, (1 << 31) - 1)])
+def test_cache_counts_beyond_the_size_arithmetic(lib, n_seqs, heads, ctx):
+    """2^40 and more (sequence, kv head, slot) triples are refused, before any
+    product of them is a size: at the last two, a workspace of 2^64 bytes."""
+    C = ctypes.byref(_cache(n_seqs=n_seqs, n_kv_heads=heads, max_ctx=ctx))
+    assert lib.li_kv_evict_workspace_size(C, (ctx + 1) // 2) == 0 == lib.li_attn_kv_workspace_size(C, heads)
+    assert lib.li_launch_kv_evict(C, P, (ctx + 1) // 2, 0, 0, P, 1 << 62, None) == BAD_SHAPE
+    assert lib.li_launch_attn_kv_decode(C, P, 128, heads, 0.1, P, 1.0, P, 1 << 62, None) == BAD_SHAPE
+    assert lib.li_launch_kv_append(C, None, 0, None, 0, None, 0, 0, P, 128, P, 128, P, None, None, 0, None) == BAD_SHAPE
