@@ -443,7 +443,8 @@ int li_launch_attn_layer_decode(const li_attn_layer * L,
 /* Rotary positions (see li_rope) of x [n_tokens][n_heads][head_dim]: strides
  * in elements between tokens and between heads, the head's values contiguous.
  * dst has its own strides and the element type of x; dst may be x itself with
- * the same strides, and must not overlap it in any other way. pos [n_tokens]
+ * the same strides, and must not overlap it in any other way; dst's own rows
+ * must not overlap (strides below head_dim are refused). pos [n_tokens]
  * int32 in device memory, any value (a negative one turns backwards).
  * transpose != 0 applies the transposed matrix: the gradient of the rotation,
  * and its inverse where the magnitude m is 1. Turning cached keys by a
@@ -461,7 +462,7 @@ int li_launch_rope(const li_rope * R, int dtype, const void * x, void * dst, con
  * [n_tokens][n_q_heads][D] is written rotated to q_out (which may be q with
  * the same stride; q NULL: no queries), k and v [n_tokens][n_kv_heads][D] are
  * rounded to f16 into their cache rows (k rotated; R NULL: nothing rotates);
- * strides in elements between tokens, heads contiguous. Where the cache holds
+ * strides in elements between tokens, heads contiguous, q_out's rows apart. Where the cache holds
  * them, weight is set to 0 and slot_pos to pos[t] in the new slots. len is
  * not changed. A sequence or slot outside the cache writes nothing there and
  * li_device_status() reports LI_ERR_BAD_ARG (its q is still rotated). Two

@@ -339,6 +339,9 @@ int vec_of(int e, const void *p, int64_t stride, int elem) {
     return e;
 }
 
+// Rows of `row` elements, `stride` apart: neighbours would overlap.
+bool overlap(int n, int64_t stride, int64_t row) { return n > 1 && stride < row && stride > -row; }
+
 int elem_size(int dtype) {
     return dtype == LI_DTYPE_F32 ? 4 : dtype == LI_DTYPE_F16 || dtype == LI_DTYPE_BF16 ? 2 : 0;
 }
@@ -358,6 +361,8 @@ extern "C" int li_launch_rope(const li_rope *R, int dtype, const void *x, void *
     if (const int rc = rope_args(R, &j.r)) return rc;
     if ((uintptr_t)x % es || (uintptr_t)dst % es || (uintptr_t)pos & 3u) return LI_ERR_MISALIGNED;
     if (n_tokens == 0 || n_heads == 0) return 0;
+    if (overlap(n_tokens, dst_token_stride, R->head_dim) || overlap(n_heads, dst_head_stride, R->head_dim))
+        return LI_ERR_BAD_SHAPE;
     j.x = x; j.dst = dst; j.pos = pos;
     j.x_ts = x_token_stride; j.x_hs = x_head_stride; j.d_ts = dst_token_stride; j.d_hs = dst_head_stride;
     j.n_tokens = n_tokens; j.heads = n_heads; j.D = R->head_dim;
@@ -392,6 +397,7 @@ extern "C" int li_launch_kv_append(const li_kv_cache *C, const li_rope *R, int d
     j.x = q; j.dst = q_out; j.pos = pos;
     j.Hq = q ? n_q_heads : 0; j.Hkv = C->n_kv_heads; j.D = C->head_dim;
     if ((int64_t)j.Hq + 2ll * j.Hkv > (1 << 24)) return LI_ERR_BAD_SHAPE;
+    if (q && overlap(n_tokens, q_out_stride, (int64_t)j.Hq * j.D)) return LI_ERR_BAD_SHAPE;
     j.x_ts = q_stride; j.x_hs = j.D; j.d_ts = q_out_stride; j.d_hs = j.D;
     j.n_tokens = n_tokens; j.heads = j.Hq + 2 * j.Hkv;
     j.sin_sign = 1.f;

@@ -305,3 +305,21 @@ def test_cache_counts_beyond_the_size_arithmetic(lib, n_seqs, heads, ctx):
     assert lib.li_launch_kv_evict(C, P, (ctx + 1) // 2, 0, 0, P, 1 << 62, None) == BAD_SHAPE
     assert lib.li_launch_attn_kv_decode(C, P, 128, heads, 0.1, P, 1.0, P, 1 << 62, None) == BAD_SHAPE
     assert lib.li_launch_kv_append(C, None, 0, None, 0, None, 0, 0, P, 128, P, 128, P, None, None, 0, None) == BAD_SHAPE
+
+
+def test_outputs_whose_rows_overlap(lib):
+    """A destination whose rows lie on one another (an expanded tensor, say)
+    would be written by several threads at once; sources may repeat."""
+    R, C = ctypes.byref(_rope()), ctypes.byref(_cache())
+
+    def rope(n, heads, ts, hs):
+        return lib.li_launch_rope(R, 0, P, P, P, n, heads, 0, 0, ts, hs, 0, None)
+
+    assert rope(2, 3, 0, 128) == BAD_SHAPE and rope(2, 3, 384, 0) == BAD_SHAPE
+    assert rope(2, 3, 127, 256) == BAD_SHAPE and rope(2, 3, 384, -64) == BAD_SHAPE
+    assert rope(1, 3, 0, 100) == BAD_SHAPE and rope(9, 1, -100, 0) == BAD_SHAPE
+
+    def append(n, stride):
+        return lib.li_launch_kv_append(C, R, 0, P, 512, P, stride, 4, P, 256, P, 256, P, None, None, n, None)
+
+    assert append(2, 0) == BAD_SHAPE and append(3, 511) == BAD_SHAPE and append(2, -384) == BAD_SHAPE
