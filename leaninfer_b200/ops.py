@@ -329,6 +329,8 @@ class AttnLayerDecode:
         if x.shape != (cache.n_seqs, self.L.hidden) or y.shape != x.shape or x.dtype != y.dtype or \
                 x.dtype != torch.float32:
             raise ValueError(f"x, y: expected fp32 [{cache.n_seqs}, {self.L.hidden}]")
+        if cache.n_seqs == 0:
+            return y
         lib, L = _lib.load(), self.L
         ws = workspace if workspace is not None else cache._workspace(
             ("layer", L.hidden, L.n_q_heads, L.w_in_type, L.w_out_type), lambda: int(lib.li_attn_layer_kv_workspace_size(ctypes.byref(self.L), cache.ref)))

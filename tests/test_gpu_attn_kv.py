@@ -228,3 +228,17 @@ def test_rope_node(cuda, dt, mode):
     ref = ops.rope(R, x, pos)
     torch.cuda.synchronize()
     assert torch.equal(out, ref)
+
+
+def test_layer_step_of_an_empty_batch(cuda):
+    """No sequences: nothing happens, as in append, decode and evict."""
+    import torch
+    from leaninfer_b200 import ops, synth
+    w = synth.attn_layer(rng(7500), hidden=1024, n_q_heads=8, n_kv_heads=2, wtype=12)
+    layer = _layer(cuda, w)
+    z = lambda *s, dt=torch.float32: torch.empty(*s, device=cuda, dtype=dt)
+    none = z(0, dt=torch.int32)
+    cache = ops.KVCache(z(0, 16, 2, 128, dt=torch.float16), z(0, 16, 2, 128, dt=torch.float16), none)
+    y = z(0, 1024)
+    assert layer.step_kv(z(0, 1024), y, cache, none) is y
+    assert ops.device_status() == 0
