@@ -700,3 +700,164 @@ def test_evict_workspace_does_not_grow_with_budgets(cuda):
         cache.evict(pos, budget)
         assert t["lens"].tolist() == [budget] * 2
         assert torch.cuda.memory_allocated() == before
+
+
+# --------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("pad", [0, 8, 12, 2, 1])
+def test_append_with_every_vector_width(cuda, dt, layout, pad):
+    """Prompts of 700 tokens out of projections whose row length allows
+    vectors of 8, 4, 2 or 1 values: blocks of several tokens, several rounds,
+    and tokens split over the heads."""
+    from leaninfer_b200 import ops
+    from oracle import kv
+    r = rng(930 + pad)
+    B, ctx, Hkv, G, each = 3, 710, 3, 4, 700
+    c, t, cache = _cache(r, cuda, B, ctx, Hkv, [705, 700, 710], stale=None)
+    kw = dict(head_dim=128, rope_dim=64 if layout == "half" else 128, layout=layout, theta=1e6)
+    first = np.array([5, 0, 10])
+    seq, slot = np.repeat(np.arange(B), each), (first[:, None] + np.arange(each)).reshape(-1)
+    n = B * each
+    pos = (slot + 1000).astype(np.int32)
+    proj = T(r.standard_normal((n, (G + 2) * Hkv * 128 + pad)).astype(np.float32), cuda).to(_torch_dt(dt))
+    cut = lambda a, b: proj[:, a * 128:b * 128].view(n, b - a, 128)
+    q, k, v = cut(0, G * Hkv), cut(G * Hkv, (G + 1) * Hkv), cut((G + 1) * Hkv, (G + 2) * Hkv)
+    got = cache.append(k, v, T(pos, cuda), q=q, rope=ops.Rope(**kw), seq=T(seq.astype(np.int32), cuda),
+                       slot=T(slot.astype(np.int32), cuda))
+    q64, k64, v64 = (a.double().cpu().numpy() for a in (q, k, v))
+    _check_rope(got, kv.rope(q64, pos, **kw), q64, 1.0, dt, "q")
+    k_ref = kv.rope(k64, pos, **kw)
+    kc, vc = t["k"].cpu().numpy(), t["v"].cpu().numpy()
+    tol = 2.0 ** -20 * np.abs(k64).max() + 2.0 ** -25
+    assert np.all(np.abs(kc[seq, slot].astype(np.float64) - k_ref) <= tol + 2.0 ** -11 * np.abs(k_ref))
+    assert np.all(np.abs(vc[seq, slot].astype(np.float64) - v64) <= 2.0 ** -11 * np.abs(v64) + 2.0 ** -25)
+    rest = np.ones((B, ctx), bool)
+    rest[seq, slot] = False
+    assert np.array_equal(kc[rest], c["k"][rest]) and np.array_equal(vc[rest], c["v"][rest])
+    w, sp = t["weight"].cpu().numpy(), t["slot_pos"].cpu().numpy()
+    assert np.all(w[seq, :, slot] == 0) and np.all(sp[seq, :, slot] == pos[:, None])
+    rest_h = np.broadcast_to(rest[:, None], w.shape)
+    assert np.array_equal(w[rest_h], c["weight"][rest_h]) and np.array_equal(sp[rest_h], c["slot_pos"][rest_h])
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("B,P", [(4500, 13), (4500, 100), (2049, 29)])
+def test_many_sequences_over_a_prefix(cuda, B, P):
+    """More sequences than the length scan has entries, over a prefix that goes
+    with the own tokens (4500 x 13 x 512 bytes are below 30 MB) and over one
+    that the tensor-core kernel takes."""
+    r = rng(940 + P)
+    lens = r.integers(0, 6, B).astype(np.int32)
+    lens[100:1300] = 0
+    _attn_check(cuda, r, B, P, 5, lens, 1, 2, decay=0.5)
+
+
+@pytest.mark.parametrize("B,P,ctx,limit", [(8, 131072, 16, 4e-6), (16, 0, 32768, 2.5e-6)])
+def test_long_sums_stay_as_exact_as_fp32(cuda, B, P, ctx, limit):
+    """Sums over many tokens, normwise against 64 bits. The tensor cores round
+    towards zero, half a unit (2^-24 of the sum at most) a product on average;
+    what that adds up to is bounded by how long a sum stays with them.
+      prefix  64 products (4 tiles of 128 tokens, hi and lo parts, 16 tokens
+              each) to a sum, whose partial sums have 2/3 of its size on
+              average: 64 * 2^-24 * 2/3 = 2.5e-6. The score's 8 hi products:
+              8 * 2^-24 * 1.5 (q's size) = 7e-7. Limit 4e-6; a sum left alone over
+              a block's 28 tiles would be off by 1.8e-5.
+      own     16 steps to a sum: 16 * 2^-24 * 2/3 = 6.4e-7, scores 7e-7, the
+              split of p 2^-23. Limit 2.5e-6; left alone over a warp's 221 steps:
+              8.8e-6.
+    """
+    import torch
+    from leaninfer_b200 import ops
+    Hkv, G = 8, 4
+    g = torch.Generator(device=cuda).manual_seed(950 + B)
+    n16 = lambda *s: torch.randn(*s, generator=g, device=cuda, dtype=torch.float16)
+    k, v = n16(B, ctx, Hkv, 128), n16(B, ctx, Hkv, 128)
+    kp, vp = (n16(P, Hkv, 128), n16(P, Hkv, 128)) if P else (None, None)
+    q = 1.5 * torch.randn(B, Hkv * G, 128, generator=g, device=cuda)
+    cache = ops.KVCache(k, v, torch.full((B,), ctx, device=cuda, dtype=torch.int32), k_prefix=kp, v_prefix=vp)
+    got = cache.decode(q).double()
+    ref = torch.empty_like(got)
+    for s in range(B):
+        for j in range(Hkv):
+            kk, vv = ((torch.cat([p[:, j], o[s, :, j]]) if P else o[s, :, j]).double() for p, o in ((kp, k), (vp, v)))
+            sc = q[s, j * G:(j + 1) * G].double() @ kk.T * 128 ** -0.5
+            ref[s, j * G:(j + 1) * G] = sc.softmax(-1) @ vv
+    err = float((got - ref).norm() / ref.norm())
+    assert err <= limit, f"{err:.2e}"
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("P", [100, 3000])
+def test_first_calls_inside_a_capture(cuda, P):
+    """Append, decode and evict of a cache that has made no call yet, captured
+    (the workspaces come from the capture's pool), replayed and then called
+    eagerly with other work in between: the bits of eager calls alone."""
+    import torch
+    from leaninfer_b200 import ops
+    r = rng(960)
+    B, ctx, Hkv, G, budget = 12, 40, 2, 4, 30
+    R = ops.Rope(head_dim=128, rope_dim=64, theta=1e6)
+    c, t, _ = _cache(r, cuda, B, ctx, Hkv, [36] * B, P, stale=None)
+    q, k, v = (T(r.standard_normal((B, h, 128)).astype(np.float32), cuda) for h in (Hkv * G, Hkv, Hkv))
+    pos = T(np.full(B, P + 36, np.int32), cuda)
+
+    def fresh():
+        d = {n: x.clone() for n, x in t.items()}
+        cache = ops.KVCache(d["k"], d["v"], d["lens"], k_prefix=d["kp"], v_prefix=d["vp"], weight=d["weight"],
+                            slot_pos=d["slot_pos"])
+        return d, cache, torch.zeros_like(q), torch.zeros_like(q)
+
+    def run(d, cache, qr, out):
+        cache.append(k, v, pos, q=q, rope=R, q_out=qr)
+        cache.decode(qr, out=out)
+        cache.evict(pos, budget, n_sink=2, n_recent=4)
+
+    eager, graphed = fresh(), fresh()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(*graphed)
+    for turn in range(3):
+        run(*eager)
+        noise = [torch.randn(1 << 20, device=cuda) for _ in range(4)]      # what the allocator hands out now
+        if turn == 2:
+            run(*graphed)
+        else:
+            graph.replay()
+        del noise
+        for name in t:
+            assert torch.equal(eager[0][name], graphed[0][name]), (turn, name)
+        assert torch.equal(eager[3], graphed[3])
+    assert ops.device_status() == 0
+
+
+def test_repeated_sources(cuda):
+    """Sources may repeat: one q for every sequence, one head for every head."""
+    import torch
+    from leaninfer_b200 import ops
+    r = rng(970)
+    R = ops.Rope(head_dim=64, rope_dim=32, theta=1e5)
+    one = T(r.standard_normal((1, 1, 64)).astype(np.float32), cuda)
+    pos = T(np.arange(9, dtype=np.int32), cuda)
+    assert torch.equal(ops.rope(R, one.expand(9, 5, 64), pos), ops.rope(R, one.expand(9, 5, 64).contiguous(), pos))
+    with pytest.raises(ops.LeanInferError):
+        ops.rope(R, torch.zeros(9, 5, 64, device=cuda), pos, out=one.expand(9, 5, 64).clone()[:1].expand(9, 5, 64))
+    for B, P in ((4, 20), (20, 2000)):
+        c, t, cache = _cache(r, cuda, B, 30, 2, [30] * B, P)
+        q = T(r.standard_normal((1, 8, 128)).astype(np.float32), cuda).expand(B, 8, 128)
+        assert torch.equal(cache.decode(q, decay=0.0), cache.decode(q.contiguous(), decay=0.0))
+    assert ops.device_status() == 0
+
+
+def test_launches_follow_the_current_stream(cuda):
+    """The stream handle that the wrappers pass is the current stream's."""
+    import torch
+    from leaninfer_b200 import ops
+    assert ops._stream() == torch.cuda.current_stream().cuda_stream
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert ops._stream() == side.cuda_stream != torch.cuda.default_stream().cuda_stream
+    x = torch.zeros(1, device=cuda)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        x += 1
+        assert ops._stream() == torch.cuda.current_stream().cuda_stream
