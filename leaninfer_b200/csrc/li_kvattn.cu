@@ -1298,7 +1298,12 @@ size_t plan(const li_kv_cache *C, int n_q_heads, KvAttnArgs *a, size_t *off /* [
     a->max_ctx = C->max_ctx; a->n_prefix = C->n_prefix;
     const int64_t pairs = (int64_t)a->B * a->Hkv;
     // A prefix that is little to read even once per sequence (30 MB: about 5 us), or that has one reader, goes with
-    // the own tokens: one kernel less, and no tile of 128 rows for a few.
+    // the own tokens: one kernel less, and no tile of 128 rows for a few. Us with the prefix kernel and without, 100
+    // own tokens, caches cold: 4 sequences x 32 heads 20 and 16 at 256 tokens (4 MB), 26 and 20 at 1919 (30 MB), 28
+    // and 24 at 4000 (62 MB), even at 8000; 16 sequences 22 and 20 at 480 (30 MB), 24 and 24 at 1000, 25 and 33 at
+    // 2000 (125 MB); 64 sequences x 40 heads even at 30 tokens (7 MB), 23 and 24 at 119 (30 MB), 23 and 28 at 250. One
+    // sequence: 20 and 15 at 512 tokens, 119 and 115 at 131072 with 8 kv heads, even with 4, but 41 and 57 with one,
+    // whose 8192 steps are few for 1184 warps.
     if (a->n_prefix > 0 && (a->B == 1 || pairs * a->n_prefix <= (30ll << 20) / (4 * kKvD))) {
         a->lead = a->n_prefix;
         a->n_prefix = 0;
@@ -1312,7 +1317,10 @@ size_t plan(const li_kv_cache *C, int n_q_heads, KvAttnArgs *a, size_t *off /* [
         a->n_tt = (a->n_prefix + kPreTok - 1) / kPreTok;
         const int64_t cost = (int64_t)a->Hkv * a->n_rt * a->n_tt;
         if (cost >= (1ll << 30)) return 0;
-        // two row tiles share the K and V tiles they read, unless that leaves SMs idle
+        // Two row tiles share the K and V tiles they read, unless that leaves SMs idle. Us with one and with two: 33
+        // and 35 at 1.3 units an SM (64 sequences x 1024 x 40 heads), 38 and 39 at 2.6, 53 and 53 at 10; where the
+        // prefix is beyond L2 or the rows are many, 190 and 181 (64 x 65536), 369 and 346 (512 x 16384), though 661 and
+        // 703 at 256 x 65536.
         a->per_group = a->n_rt > 1 && cost >= 2ll * sms ? 2 : 1;
         a->n_grp = (a->n_rt + a->per_group - 1) / a->per_group;
         a->slots = a->per_group == 2 ? kPreSlots2 : kPreSlots1;

@@ -26,7 +26,10 @@ namespace li {
 namespace {
 
 constexpr int kSelCacheMax = 48 * 1024;     // keys held in shared memory up to this many slots
-constexpr int kSelWide = 8192;              // from this many slots on, blocks of 1024 threads, below 512
+// From this many slots on, blocks of 1024 threads, below of 512, two an SM. Us with 512 and with 1024, caches cold: 1
+// sequence x 8 heads 16 and 17 at 4352 slots, 24 and 17 at 8192; 2 x 8 at 18000 45 and 33; 64 x 8 at 4352 slots 29
+// and 47 (3.5 blocks an SM), at 8192 48 and 48.
+constexpr int kSelWide = 8192;
 constexpr int kSelMoves = 256;              // moves that kv_select makes itself
 constexpr int kBins = 2048;                 // of a digit
 constexpr int kMovePer = 8;                 // moves of a warp in flight

@@ -46,7 +46,8 @@ int rope_args(const li_rope *R, RopeArgs *a) {
     a->rope_dim = d;
     a->mag = (float)mag;
     a->factors = R->freq_factors;
-    // theta^(-2i/d) by repeated products: 256 of them are off by 2^-45, far below a float's 2^-24
+    // theta^(-2i/d) by repeated products: off by 2^-46 of the value at worst (256 products), and by 2^-53 of a turn a
+    // position, since the frequencies shrink meanwhile (bases of 100 and more)
     const double ratio = d > 0 ? exp(-2.0 / d * lt) : 1.0;
     double f = 1.0 / two_pi;
     for (int i = 0; i < d / 2; ++i, f *= ratio) {

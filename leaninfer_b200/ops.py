@@ -433,7 +433,9 @@ class KVCache:
     in use, which the caller advances before a step's append; an optional
     shared prefix fp16 [n_prefix, n_kv_heads, 128]; weight fp32 and slot_pos
     int32 [n_seqs, n_kv_heads, max_ctx] for the eviction. Workspaces are kept
-    by the object; calls that overlap on the GPU need an object each."""
+    by the object, and captured graphs hold their addresses: calls and replays
+    that overlap on the GPU need an object each, and the object has to live as
+    long as the graphs."""
 
     def __init__(self, k, v, len, *, k_prefix=None, v_prefix=None, weight=None, slot_pos=None):
         n, ctx, heads, dim = k.shape
@@ -470,9 +472,9 @@ class KVCache:
 
     def append(self, k, v, pos, *, q=None, rope: Rope | None = None, seq=None, slot=None, q_out=None):
         """Appends k, v [tokens, n_kv_heads, 128] (k rotated to pos) at
-        (seq[t], slot[t]); without seq, token t is sequence t's, without slot
-        it goes to slot len - 1. Returns q rotated (q_out, which may be q), or
-        None without q."""
+        (seq[t], slot[t]), no two tokens at the same place; without seq, token
+        t is sequence t's, without slot it goes to slot len - 1. Returns q
+        rotated (q_out, which may be q), or None without q."""
         n, dt, dim = k.shape[0], k.dtype, self.head_dim
         if dt not in _DTYPES:
             raise ValueError(f"k: {dt} is not fp32, fp16 or bf16")
