@@ -1302,8 +1302,8 @@ size_t plan(const li_kv_cache *C, int n_q_heads, KvAttnArgs *a, size_t *off /* [
     // own tokens, caches cold: 4 sequences x 32 heads 20 and 16 at 256 tokens (4 MB), 26 and 20 at 1919 (30 MB), 28
     // and 24 at 4000 (62 MB), even at 8000; 16 sequences 22 and 20 at 480 (30 MB), 24 and 24 at 1000, 25 and 33 at
     // 2000 (125 MB); 64 sequences x 40 heads even at 30 tokens (7 MB), 23 and 24 at 119 (30 MB), 23 and 28 at 250. One
-    // sequence: 20 and 15 at 512 tokens, 119 and 115 at 131072 with 8 kv heads, even with 4, but 41 and 57 with one,
-    // whose 8192 steps are few for 1184 warps.
+    // sequence: 20 and 15 at 512 tokens, 119 and 115 at 131072 with 8 kv heads, even with 4, but 41 and 57 with
+    // one.
     if (a->n_prefix > 0 && (a->B == 1 || pairs * a->n_prefix <= (30ll << 20) / (4 * kKvD))) {
         a->lead = a->n_prefix;
         a->n_prefix = 0;

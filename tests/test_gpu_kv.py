@@ -690,11 +690,14 @@ def test_queries_at_the_ends_of_fp32(cuda, B, P, kw):
 def test_evict_workspace_does_not_grow_with_budgets(cuda):
     """One workspace serves every budget: a host that varies it allocates no
     more, and the address that a captured eviction holds stays in use."""
+    import gc
+
     import torch
     r = rng(920)
     c, t, cache = _cache(r, cuda, 2, 600, 2, [600, 600], stale=None)
     pos = T(np.full(2, 599, np.int32), cuda)
     cache.evict(pos, 599)
+    gc.collect()                           # what earlier tests left is not freed in between
     before = torch.cuda.memory_allocated()
     for budget in (590, 580, 400, 301, 300, 299, 200, 100, 7, 0):
         cache.evict(pos, budget)
